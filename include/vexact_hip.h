@@ -99,6 +99,27 @@ int vx_logprobs_bwd(const void* logits, const int64_t* labels, const float* out,
 int vx_logprobs_static(const void* logits, const int64_t* labels, float* out, int64_t* tokens_out, int dtype,
                        int64_t rows, int64_t n, int64_t x_stride, hipStream_t stream);
 
+/* Log-probabilities of given tokens from the hidden states [T, H] and the output projection [V, H] (both bf16, H
+ * contiguous, H a multiple of 8, 16-byte aligned rows): x = scale * hidden weight^T (scale = 1 / temperature) in fp32,
+ * lse = logsumexp(x), out[i] = x[i, labels[i]] - lse[i]; neither the logits nor a rounded copy of them reaches memory.
+ * out and lse [T] fp32, either may be null. A label outside [0, V) gives NaN (as vx_logprobs). The fold over the
+ * vocabulary is at fixed positions: a row's bits do not depend on T. They are not the bits of vx_logprobs on a bf16
+ * tensor of logits, which rounds every logit. No counterpart in the reference, whose logprob takes logits
+ * (standalone_logprobs.py:28-55).
+ * The backward recomputes x in pieces of the vocabulary: d_hidden [T, H] and / or d_weight [V, H] (bf16, row strides
+ * multiples of 4, either may be null), from the forward's lse and d_out [T] fp32. Rows whose label is outside the
+ * vocabulary have no gradient, whatever their d_out. The derivative of each logit is rounded to bf16 once before the
+ * two products, which accumulate in fp32; no atomics, results repeat bit for bit. T <= 2^32 / 16384 rows. */
+int64_t vx_vocab_logprobs_workspace_bytes(int64_t T, int64_t V);
+int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* labels, float* out, float* lse, int64_t T,
+                      int64_t V, int64_t H, int64_t ldh, int64_t ldw, float scale, void* workspace,
+                      int64_t workspace_bytes, hipStream_t stream);
+int64_t vx_vocab_logprobs_bwd_workspace_bytes(int64_t T, int64_t V, int64_t H);
+int vx_vocab_logprobs_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* lse,
+                          const float* d_out, void* d_hidden, void* d_weight, int64_t T, int64_t V, int64_t H,
+                          int64_t ldh, int64_t ldw, int64_t ld_dh, int64_t ld_dw, float scale, void* workspace,
+                          int64_t workspace_bytes, hipStream_t stream);
+
 /* ---- dense GEMM ----------------------------------------------------------------------- */
 
 /* C[M,N] = X[M,K] * W[N,K]^T (+ bias[N]), bf16 in/out, fp32 accumulate, K ascending, no split-K.

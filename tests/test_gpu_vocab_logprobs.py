@@ -1,0 +1,280 @@
+"""Log-probabilities from hidden states and their gradients against a plain implementation in 64 bits.
+
+Tolerances. Forward: a logit is a sum of H products accumulated in fp32; its rounding errors add like independent ones,
+so 8 sqrt(H) 2^-24 sum_k |h_k w_k| covers a logit, and twice that a log-probability (its own logit and the lse, which
+moves by at most the largest logit error), beside a few fp32 steps of the result. Gradients: every entry of the logits'
+derivative is rounded to bf16 once (half a step, 2^-8 relative), which moves an output by at most 2^-8 sum |dx| |w|;
+the result is rounded to bf16 once more (2^-8 of itself); 2^-11 of the same sum covers the fp32 part (a probability's
+relative error is that of its exponent's argument, below 2^-13 here) and the accumulation.
+"""
+
+import pytest
+import torch
+
+from vexact_amd import ops
+from vexact_amd.batch_invariant_ops.standalone_logprobs import logprobs_from_hidden
+
+from .util import assert_bitwise
+
+gpu = pytest.mark.gpu
+
+
+def make(T, V, H, seed=0, ignored=0, spread=1.8):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(T, H, generator=g).to(torch.bfloat16)
+    w = (spread / H**0.5 * torch.randn(V, H, generator=g)).to(torch.bfloat16)
+    y = torch.randint(0, V, (T,), generator=g)
+    y[torch.randperm(T, generator=g)[:ignored]] = -100
+    return h, w, y
+
+
+def reference(h, w, y, temperature=1.0, d=None):
+    h64, w64 = h.double(), w.double()
+    x = h64 @ w64.t() / temperature
+    lse = torch.logsumexp(x, 1)
+    ok = (y >= 0) & (y < w.shape[0])
+    at = y.clamp(0, w.shape[0] - 1)
+    lp = torch.where(ok, x.gather(1, at[:, None])[:, 0] - lse, torch.nan)
+    if d is None:
+        return lp, lse
+    dd = torch.where(ok, d.double(), 0.0) / temperature
+    dx = -torch.exp(x - lse[:, None]) * dd[:, None]
+    dx[torch.arange(len(y)), at] += dd
+    return lp, lse, dx, dx @ w64, dx.t() @ h64
+
+
+def check_forward(h, w, y, out, lse, temperature=1.0):
+    lp_ref, lse_ref = reference(h, w, y, temperature)
+    mass = (h.double().abs() @ w.double().abs().t()).max() / temperature
+    tol = 16 * h.shape[1] ** 0.5 * 2.0**-24 * mass + 4 * 2.0**-24 * lse_ref.abs().max() + 2.0**-20
+    assert torch.equal(torch.isnan(out.cpu()), torch.isnan(lp_ref))
+    ok = ~torch.isnan(lp_ref)
+    assert (out.cpu().double() - lp_ref)[ok].abs().max() <= tol if ok.any() else True
+    assert (lse.cpu().double() - lse_ref).abs().max() <= tol
+
+
+# rows on both sides of the kernels' tile heights; vocabularies that end inside a strip, a tile and a segment; depths
+# that are and are not a multiple of the wide kernel's step
+SHAPES = [(1, 1, 8), (1, 5, 64), (3, 64, 64), (7, 257, 72), (64, 1000, 128), (65, 1000, 128), (100, 1024, 136), (129, 8192, 64),
+          (300, 8193, 192), (257, 20011, 128), (513, 16449, 256), (30, 20011, 520)]
+
+
+@gpu
+@pytest.mark.parametrize("T,V,H", SHAPES)
+def test_forward(T, V, H):
+    h, w, y = make(T, V, H, seed=T, ignored=T // 5)
+    if T > 2:
+        y[0], y[1] = V - 1, V  # the last token, and one past it
+    out, lse = ops.vocab_logprobs(h.cuda(), w.cuda(), y.cuda(), 0.7)
+    check_forward(h, w, y, out, lse, 0.7)
+
+
+@gpu
+@pytest.mark.parametrize("T,V,H", SHAPES)
+def test_backward(T, V, H):
+    h, w, y = make(T, V, H, seed=T + 1, ignored=T // 5)
+    d = torch.randn(T, generator=torch.Generator().manual_seed(3))
+    hg, wg, yg = h.cuda(), w.cuda(), y.cuda()
+    _, lse = ops.vocab_logprobs(hg, wg, yg, 1.3)
+    dh, dw = ops.vocab_logprobs_backward(hg, wg, yg, lse, d.cuda(), 1.3)
+    _, _, dx, dh_ref, dw_ref = reference(h, w, y, 1.3, d)
+    slack = 2.0**-8 + 2.0**-11
+    tol_h = slack * (dx.abs() @ w.double().abs()) + 2.0**-8 * dh_ref.abs() + 1e-30
+    tol_w = slack * (dx.abs().t() @ h.double().abs()) + 2.0**-8 * dw_ref.abs() + 1e-30
+    assert ((dh.cpu().double() - dh_ref).abs() <= tol_h).all()
+    assert ((dw.cpu().double() - dw_ref).abs() <= tol_w).all()
+    # one gradient alone is the same
+    assert_bitwise(ops.vocab_logprobs_backward(hg, wg, yg, lse, d.cuda(), 1.3, need_weight=False)[0], dh, "d_hidden alone")
+    assert_bitwise(ops.vocab_logprobs_backward(hg, wg, yg, lse, d.cuda(), 1.3, need_hidden=False)[1], dw, "d_weight alone")
+
+
+@gpu
+@pytest.mark.parametrize("V,H", [(20011, 128), (1000, 72)])
+def test_rows_do_not_depend_on_the_batch(V, H):
+    h, w, y = (t.cuda() for t in make(600, V, H, seed=5))
+    out, lse = ops.vocab_logprobs(h, w, y)
+    d = torch.randn(600, generator=torch.Generator().manual_seed(1)).cuda()
+    dh, _ = ops.vocab_logprobs_backward(h, w, y, lse, d)
+    for a, b in ((0, 1), (17, 24), (100, 164), (100, 165), (300, 600)):
+        o2, l2 = ops.vocab_logprobs(h[a:b], w, y[a:b])
+        assert_bitwise(o2, out[a:b], f"rows {a}..{b}")
+        assert_bitwise(l2, lse[a:b], f"lse of rows {a}..{b}")
+        dh2, _ = ops.vocab_logprobs_backward(h[a:b], w, y[a:b], l2, d[a:b], need_weight=False)
+        assert_bitwise(dh2, dh[a:b], f"d_hidden of rows {a}..{b}")
+
+
+@gpu
+def test_pieces_of_the_vocabulary_change_nothing():
+    """Enough rows for several pieces: the gradient of the first rows is that of a one-piece call."""
+    V, H, T = 40000, 128, 12000
+    h, w, y = (t.cuda() for t in make(T, V, H, seed=6))
+    out, lse = ops.vocab_logprobs(h, w, y)
+    d = torch.randn(T, generator=torch.Generator().manual_seed(2)).cuda()
+    dh, dw = ops.vocab_logprobs_backward(h, w, y, lse, d)
+    few = ops.vocab_logprobs_backward(h[:200], w, y[:200], lse[:200], d[:200], need_weight=False)[0]
+    assert_bitwise(dh[:200], few, "first rows")
+    # the weight gradient of all rows against products of the logits' derivative in 32 bits
+    x = h.float() @ w.float().t()
+    dx = -torch.exp(x - lse[:, None]) * d[:, None]
+    dx.scatter_add_(1, y[:, None], d[:, None])
+    ref, mass = dx.t() @ h.float(), dx.abs().t() @ h.float().abs()
+    assert ((dw.float() - ref).abs() <= (2.0**-8 + 2.0**-10) * mass + 2.0**-8 * ref.abs()).all()
+
+
+@gpu
+def test_strided_operands_and_special_rows():
+    T, V, H = 70, 500, 128
+    h, w, y = make(T, V, H, seed=8)
+    hb, wb = torch.zeros(T, H + 24, dtype=torch.bfloat16).cuda(), torch.zeros(V, 2 * H, dtype=torch.bfloat16).cuda()
+    hb[:, 8 : 8 + H], wb[:, H:] = h.cuda(), w.cuda()
+    base, lse = ops.vocab_logprobs(h.cuda(), w.cuda(), y.cuda())
+    for hv, wv in ((hb[:, 8 : 8 + H], wb[:, H:]), (h.cuda().t().contiguous().t(), w.cuda()), (h.cuda(), w.cuda().t().contiguous().t())):
+        out, l2 = ops.vocab_logprobs(hv, wv, y.cuda())
+        assert_bitwise(out, base)
+        assert_bitwise(l2, lse)
+        d = torch.ones(T).cuda()
+        for a, b in zip(ops.vocab_logprobs_backward(hv, wv, y.cuda(), l2, d), ops.vocab_logprobs_backward(h.cuda(), w.cuda(), y.cuda(), lse, d)):
+            assert_bitwise(a, b)
+    # a row with a NaN is NaN, its neighbours are not touched; a huge row does not overflow
+    h2 = h.clone()
+    h2[3, 5] = float("nan")
+    h2[4] *= 1000
+    out, l2 = ops.vocab_logprobs(h2.cuda(), w.cuda(), y.cuda())
+    keep = [i for i in range(T) if i not in (3, 4)]
+    assert torch.isnan(out[3]) and torch.isnan(l2[3]) and torch.isfinite(out[4])
+    assert_bitwise(out[keep], base[keep])
+    # no rows at all; rows without any label: no gradient, whatever d_out holds
+    assert ops.vocab_logprobs(h[:0].cuda(), w.cuda(), y[:0].cuda())[0].shape == (0,)
+    dh, dw = ops.vocab_logprobs_backward(h[:0].cuda(), w.cuda(), y[:0].cuda(), l2[:0], torch.ones(0).cuda())
+    assert dh.shape == (0, H) and not dw.any()
+    none = torch.full((T,), -1).cuda()
+    assert torch.isnan(ops.vocab_logprobs(h.cuda(), w.cuda(), none)[0]).all()
+    dh, dw = ops.vocab_logprobs_backward(h.cuda(), w.cuda(), none, lse, torch.full((T,), float("nan")).cuda())
+    assert not dh.any() and not dw.any()
+
+
+@gpu
+def test_autograd_shapes_and_differences():
+    B, S, V, H = 2, 40, 700, 64
+    h, w, y = make(B * S, V, H, seed=9)
+    hg, wg, yg = h.view(B, S, H).cuda().requires_grad_(), w.cuda().requires_grad_(), y.view(B, S).cuda()
+    out = logprobs_from_hidden(hg, wg, yg, temperature=0.9)
+    assert out.shape == (B, S) and out.dtype == torch.float32
+    d = torch.randn(B, S, generator=torch.Generator().manual_seed(4)).cuda()
+    (out * d).sum().backward()
+    assert hg.grad.shape == hg.shape and wg.grad.shape == wg.shape and hg.grad.dtype == torch.bfloat16
+    ref = reference(h, w, y, 0.9, d.cpu().reshape(-1))
+    assert (hg.grad.cpu().double().view(-1, H) - ref[3]).norm() <= 2.0**-7 * ref[3].norm()
+    assert (wg.grad.cpu().double() - ref[4]).norm() <= 2.0**-7 * ref[4].norm()
+    with torch.no_grad():
+        assert_bitwise(logprobs_from_hidden(hg, wg, yg, temperature=0.9), out.detach(), "without autograd")
+    # central differences along a direction of exactly representable steps, in the function's own outputs: the remainder
+    # is a sixth of the third derivative, at most (range of the logits' change)^3 per row
+    grid = (h.float() * 8).round() / 8  # multiples of 1/8: +- 1/64 stays exact below 2, which is enforced
+    grid = grid.clamp(-1.75, 1.75)
+    step = torch.randn(B * S, H, generator=torch.Generator().manual_seed(7)).sign() / 64
+    f = lambda z: ops.vocab_logprobs(z.to(torch.bfloat16).cuda(), wg.detach(), yg.reshape(-1), 0.9)  # noqa: E731
+    mid, lse = f(grid)
+    dh, _ = ops.vocab_logprobs_backward(grid.to(torch.bfloat16).cuda(), wg.detach(), yg.reshape(-1), lse, torch.ones(B * S).cuda(), 0.9, need_weight=False)
+    slope = (dh.cpu().double() * step.double()).sum(1)
+    diff = (f(grid + step)[0] - f(grid - step)[0]).cpu().double() / 2
+    moved = (step.double() @ w.double().t()) / 0.9
+    spread = moved.max(1).values - moved.min(1).values
+    dx_mass = 2 / 0.9 * (w.double().abs().max() * step.abs().sum(1).double())  # sum |dx| <= 2 / temperature
+    tol = spread**3 / 6 + 2.0**-7 * dx_mass + 2.0**-18
+    assert ((slope - diff).abs() <= tol).all()
+    assert (slope - diff).norm() <= 0.1 * slope.norm()
+
+
+@gpu
+def test_frozen_projection_and_second_stream():
+    T, V, H = 130, 3001, 128
+    h, w, y = make(T, V, H, seed=11)
+    hg = h.cuda().requires_grad_()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    wg, yg = w.cuda(), y.cuda()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        out = logprobs_from_hidden(hg, wg, yg)
+        (g,) = torch.autograd.grad(out.sum(), hg)
+    torch.cuda.current_stream().wait_stream(stream)
+    _, lse = ops.vocab_logprobs(hg.detach(), wg, yg)
+    assert_bitwise(g, ops.vocab_logprobs_backward(hg.detach(), wg, yg, lse, torch.ones(T).cuda(), need_weight=False)[0])
+
+
+@gpu
+def test_captured_forward_and_backward_replay():
+    T, V, H = 140, 9000, 128
+    h, w, y = (t.cuda() for t in make(T, V, H, seed=12))
+    d = torch.randn(T, generator=torch.Generator().manual_seed(5)).cuda()
+
+    def step():
+        out, lse = ops.vocab_logprobs(h, w, y)
+        return (out, *ops.vocab_logprobs_backward(h, w, y, lse, d))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (21, 22, 23):
+        h2, _, y2 = make(T, V, H, seed=seed)
+        h.copy_(h2)
+        y.copy_(y2)
+        eager = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, eager):
+            assert_bitwise(a, b, f"replay on inputs {seed}")
+
+
+def test_refusals():
+    h, w, y = make(4, 10, 16)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        ops.vocab_logprobs(h, w, y)
+    with pytest.raises(ValueError, match="shape of hidden's rows"):
+        logprobs_from_hidden(h, w, y[:3])
+
+
+@gpu
+def test_refusals_on_the_gpu():
+    h, w, y = (t.cuda() for t in make(4, 10, 16))
+    for args, what in (((h.half(), w.half(), y), "bfloat16"), ((h, w[:, :8], y), "need hidden"), ((h, w, y[:3]), "one per row"),
+                       ((h, w, y.float()), "integers"), ((h[:, :12], w[:, :12], y), "multiple of 8"), ((h, w[:0], y), "V positive"),
+                       ((h, w.cpu(), y), "one device")):
+        with pytest.raises(ValueError, match=what):
+            ops.vocab_logprobs(*args)
+    for bad in (0.0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.vocab_logprobs(h, w, y, bad)
+    with pytest.raises(ValueError, match="one entry per row"):
+        ops.vocab_logprobs_backward(h, w, y, torch.zeros(3).cuda(), torch.zeros(4).cuda())
+
+
+def test_c_abi_refusals():
+    """Bad arguments come back as status codes before anything is launched (no GPU needed)."""
+    from vexact_amd import _lib
+
+    lib = _lib.load()
+    a = 4096  # an aligned non-null address that is never read
+    ok = dict(h=a, w=a, y=a, o=a, l=a, T=4, V=10, H=16, ldh=16, ldw=16, ws=a, n=1 << 20)
+
+    def fwd(**kw):
+        v = {**ok, **kw}
+        return lib.vx_vocab_logprobs(v["h"], v["w"], v["y"], v["o"], v["l"], v["T"], v["V"], v["H"], v["ldh"], v["ldw"], 1.0, v["ws"], v["n"], None)
+
+    assert fwd(T=0) == 0
+    assert fwd(h=None) == fwd(w=None) == fwd(y=None) == fwd(o=None, l=None) == fwd(T=-1) == fwd(V=0) == fwd(H=0) == -1
+    assert fwd(H=12) == fwd(ldh=12) == fwd(ldw=20) == fwd(h=a + 2) == -2
+    assert fwd(ws=None) == fwd(n=16) == fwd(ws=a + 4) == -3
+
+    def bwd(**kw):
+        v = {**ok, "dh": a, "dw": a, "g": a, "ldd": 16, **kw}
+        return lib.vx_vocab_logprobs_bwd(v["h"], v["w"], v["y"], v["l"], v["g"], v["dh"], v["dw"], v["T"], v["V"], v["H"], v["ldh"], v["ldw"],
+                                         v["ldd"], v["ldd"], 1.0, v["ws"], v["n"], None)
+
+    assert bwd(T=0) == bwd(g=None) == bwd(l=None) == bwd(dh=None, dw=None) == -1
+    assert bwd(H=12) == bwd(ldd=18) == bwd(dh=a + 4) == bwd(T=1 << 28, n=1 << 60) == -2
+    assert bwd(ws=None) == bwd(n=16) == -3

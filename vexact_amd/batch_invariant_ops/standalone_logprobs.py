@@ -38,3 +38,40 @@ def logprobs_from_logits_flash_attn(
     shape = labels.shape
     out = ops.logprobs(logits.reshape(-1, logits.shape[-1]), labels.reshape(-1))
     return out.reshape(shape)
+
+
+class _HiddenLogprobsFunction(torch.autograd.Function):
+    """Log-probabilities without logits in memory, forward and backward (``ops.vocab_logprobs``)."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, temperature):
+        flat = hidden.reshape(-1, hidden.shape[-1])
+        out, lse = ops.vocab_logprobs(flat, weight, labels, temperature)
+        ctx.save_for_backward(hidden, weight, labels, lse)
+        ctx.temperature = temperature
+        return out.reshape(labels.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        hidden, weight, labels, lse = ctx.saved_tensors
+        need_hidden, need_weight = ctx.needs_input_grad[:2]
+        d_hidden, d_weight = ops.vocab_logprobs_backward(hidden.reshape(-1, hidden.shape[-1]), weight, labels, lse, d_out,
+                                                         ctx.temperature, need_hidden=need_hidden, need_weight=need_weight)
+        return d_hidden.reshape(hidden.shape) if need_hidden else None, d_weight, None, None
+
+
+def logprobs_from_hidden(
+    hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0
+) -> torch.Tensor:
+    """Log-probabilities (fp32, shape of ``labels``) of ``labels`` under ``softmax(hidden @ weight.T / temperature)``:
+    what ``logprobs_from_logits_flash_attn`` gives, from the last hidden states ``[..., H]`` and the output projection
+    ``weight [V, H]`` (bf16) instead of ``[..., V]`` logits, which at V = 151936 are 0.3 MB a token in bf16. Under
+    autograd both operands have gradients; a label outside the vocabulary (padding) gives NaN and has none. The logits are not rounded to
+    bf16 on the way, so this is not the rollout's logprob bit for bit: score both sides with the same function where
+    that matters (a row's bits do not depend on the batch)."""
+    if hidden.shape[:-1] != labels.shape:
+        raise ValueError(f"labels must have the shape of hidden's rows, got {tuple(labels.shape)} and {tuple(hidden.shape)}")
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _HiddenLogprobsFunction.apply(hidden, weight, labels, float(temperature))
+    return ops.vocab_logprobs(hidden.reshape(-1, hidden.shape[-1]), weight, labels, temperature)[0].reshape(labels.shape)

@@ -17,7 +17,8 @@
 
 namespace vx {
 
-enum : int { EPI_PLAIN = 0, EPI_SWIGLU = 1 };
+// EPI_LSE / EPI_DLOGITS: the two passes over the logits of vocab_logprob.h, which never reach memory as logits
+enum : int { EPI_PLAIN = 0, EPI_SWIGLU = 1, EPI_LSE = 2, EPI_DLOGITS = 3 };
 
 struct GemmParams {
   const bf16_t* x;   // activations
@@ -37,6 +38,16 @@ struct GemmParams {
   const int* row_src;     // [M] row of x feeding C row i (null = identity)
   const bf16_t* row_scale;      // EPI_SWIGLU: per-row routing weight (null = none), looked up as
   const int* row_scale_idx;     //   row_scale[row_scale_idx[i]] (idx null = identity)
+  // EPI_LSE / EPI_DLOGITS (vocab_logprob.h): logits are scale * acc; column n of this launch is token vocab_base + n
+  const int64_t* labels;  // [M]
+  float2* lse_part;       // EPI_LSE: (max, sum) of 256 columns, [ceil(V / 256)][part_ld]
+  int64_t part_ld;
+  float* label_logit;     // EPI_LSE: [M], the logit of the row's label
+  const float* lse;       // EPI_DLOGITS: [M]
+  const float* d_out;     // EPI_DLOGITS: [M]
+  float scale;
+  int vocab_base;
+  int64_t tokens;         // the whole vocabulary
 };
 
 __device__ __forceinline__ float silu_f32(float g) { return g / (1.0f + expf(-g)); }

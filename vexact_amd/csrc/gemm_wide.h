@@ -32,6 +32,7 @@
 #include <type_traits>
 
 #include "gemm_core.h"
+#include "vocab_logprob.h"
 
 namespace vx {
 
@@ -297,6 +298,25 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
             if (nb + e < N) cp[e] = o[e];
         }
       }
+    } else if constexpr (EPI == EPI_LSE || EPI == EPI_DLOGITS) {
+      float2* strips = (float2*)(wd_lds + 2 * STAGE);  // EPI_LSE: [4][BM] behind the stages
+#pragma unroll
+      for (int i = 0; i < XI; i++) {
+        const int m = 16 * XI * wm + 16 * i + r16;
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          v[e] = acc[i][e >> 2][e & 3];
+          acc[i][e >> 2][e & 3] = 0.f;
+        }
+        if constexpr (EPI == EPI_LSE) vocab_strip(p, v, t.row0 + m, m < t.rows, t.n0 + 64 * wn, strips + wn * BM + m);
+        else vocab_dlogits(p, v, t.row0 + m, m < t.rows, t.n0 + 64 * wn);
+      }
+      if constexpr (EPI == EPI_LSE) {
+        // the barriers of the next tile's steps keep its strips from overwriting what is read here
+        __syncthreads();
+        if (tid < t.rows) vocab_fold_strips(p, strips + tid, BM, t.row0 + tid, t.n0);
+      }
     } else {
       // lane holds C[row0 + 16 XI wm + 16 i + r16][n0 + 64 wn + 16 g + 4 j + c]
       const int nb = t.n0 + 64 * wn + 16 * g;
@@ -346,7 +366,8 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
 template <int EPI, bool GROUPED, int XI = 8, bool PACKED = false>
 static inline bool gemm_wide_launch_t(const GemmParams& p, int64_t tiles_m, int64_t x_rows, hipStream_t stream) {
   constexpr int NOUT = (EPI == EPI_SWIGLU) ? 128 : 256;
-  constexpr int LDS = 2 * (32 * XI + WD_BN) * WD_BK * 2;  // two stages of an activation and a weight tile
+  // two stages of an activation and a weight tile, and the row statistics of four 64-column strips
+  constexpr int LDS = 2 * (32 * XI + WD_BN) * WD_BK * 2 + (EPI == EPI_LSE ? 4 * 32 * XI * 8 : 0);
   if (p.K % WD_BK != 0 || p.N <= 0 || tiles_m <= 0 || x_rows <= 0) return false;
   const int64_t lim = (int64_t)1 << 32;
   // bytes of one group's weights that a load offset must reach (PACKED: 16-row blocks of p.ldw 1 KB chunks)

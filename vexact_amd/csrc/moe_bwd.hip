@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "gemm_seg.h"
 
 namespace vx {
 
@@ -59,6 +60,9 @@ struct MoeNnParams {
   int64_t ldc;
   int N;
   const int *tile_group, *tile_row0, *tile_rows;
+  // segment form of the wide kernel (gemm_seg.h): no tile table, fp32 output
+  float* cf;
+  int M, seg_cols, cols;  // rows of a; contraction indices of a segment; valid ones in all
 };
 
 template <int GB_ROWS>
@@ -197,15 +201,26 @@ __global__ __launch_bounds__(256) void moe_gemm_nn_kernel(MoeNnParams p) {
 // MFMA row rho of weight fragment j is output column 16 j + rho of the wavefront's 64 (a lane ends up with
 // four consecutive columns per fragment). Per output element the MFMA chain is the one of the kernel above.
 // Requirements (host): K, K2 multiples of 64, 32-bit byte offsets within an operand.
+// SEG (launch_gemm_nn_segments): one product A [M, cols] W [cols, N] whose contraction is cut into segments of
+// seg_cols, each with its own fp32 output [segment][M][N]: a tile is (segment, row tile, column tile) by arithmetic,
+// its operands start seg_cols further along A's columns and W's rows. Past `cols` A holds zeros up to a multiple of
+// 64; the rows of W there are re-reads of its last one.
 // ---------------------------------------------------------------------------------------
+template <bool SEG>
 __global__ __launch_bounds__(512) void moe_gemm_nn_wide_kernel(MoeNnParams p, int tiles_m, int tiles_n) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t nw_lds[];
   constexpr int XBYTES = 256 * 64 * 2, STAGE = 2 * XBYTES;
-  const int K0 = p.K[0], Ktot = K0 + (p.a[1] ? p.K[1] : 0);
+  const int K0 = p.K[0];
+  int Ktot = K0 + (p.a[1] ? p.K[1] : 0);  // SEG: of the load stream's tile
   const int tiles = tiles_m * tiles_n;
   const int G = gridDim.x;  // multiple of 8
   const int first = (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3);
-  if (first >= tiles || p.tile_group[first / tiles_n] < 0) return;
+  const int seg_tiles = SEG ? (p.M + 255) >> 8 : 1;  // row tiles of a segment
+  if (first >= tiles) return;
+  if constexpr (!SEG) {
+    if (p.tile_group[first / tiles_n] < 0) return;
+  }
+  auto seg_steps = [&](int seg) { return (min(p.seg_cols, p.cols - seg * p.seg_cols) + 63) >> 6; };
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -222,11 +237,23 @@ __global__ __launch_bounds__(512) void moe_gemm_nn_wide_kernel(MoeNnParams p, in
                                       (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
   };
   int ld_ldw = 0;
+  int ld_valid = 0;  // SEG: contraction indices of the stream's tile
   auto set_load_tile = [&](int lin, int pair) {  // offsets and bases of operand pair `pair` on tile `lin`
     const int mt = lin / tiles_n;
-    const int row0 = p.tile_row0[mt], rows = p.tile_rows[mt], n0 = (lin - mt * tiles_n) * 256;
-    const int e = p.tile_group[mt];
-    const int* src = pair == 0 ? p.a_src : nullptr;
+    const int n0 = (lin - mt * tiles_n) * 256;
+    int row0, rows, e;
+    if constexpr (SEG) {
+      e = mt / seg_tiles;
+      row0 = (mt - e * seg_tiles) * 256;
+      rows = min(256, p.M - row0);
+      ld_valid = min(p.seg_cols, p.cols - e * p.seg_cols);
+      Ktot = (ld_valid + 63) & ~63;
+    } else {
+      row0 = p.tile_row0[mt];
+      rows = p.tile_rows[mt];
+      e = p.tile_group[mt];
+    }
+    const int* src = pair == 0 && !SEG ? p.a_src : nullptr;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int R = 8 * (wave + 8 * j) + (lane >> 3);
@@ -235,10 +262,10 @@ __global__ __launch_bounds__(512) void moe_gemm_nn_wide_kernel(MoeNnParams p, in
       ld_off[j] = (uint32_t)((sr * p.lda[pair] + ((lane & 7) ^ nn_swz_x(R)) * 8) * 2);
       const int Rw = 2 * (wave + 8 * j) + (lane >> 5);
       const int col = min(n0 + 8 * ((lane & 31) ^ gb_swz(Rw)), p.N - 8);  // columns past N re-read the last piece
-      ld_off[4 + j] = (uint32_t)(((int64_t)Rw * p.ldw[pair] + col) * 2);
+      ld_off[4 + j] = (uint32_t)(((int64_t)(SEG ? min(Rw, ld_valid - 1) : Rw) * p.ldw[pair] + col) * 2);
     }
     ld_ldw = __builtin_amdgcn_readfirstlane((int)p.ldw[pair]);
-    ld_xb = uniform_ptr(p.a[pair]);
+    ld_xb = uniform_ptr(p.a[pair] + (SEG ? (int64_t)e * p.seg_cols : 0));
     ld_wb = uniform_ptr(p.w[pair] + (int64_t)e * p.w_gstride[pair]);
   };
   int ld_lin = first, ld_k = 0;
@@ -254,12 +281,20 @@ __global__ __launch_bounds__(512) void moe_gemm_nn_wide_kernel(MoeNnParams p, in
     ld_k += 64;
     ld_xb += 64;
     ld_wb += 64 * ld_ldw;
-    if (ld_k == K0 && Ktot > K0) set_load_tile(ld_lin, 1);
+    if constexpr (!SEG) {
+      if (ld_k == K0 && Ktot > K0) set_load_tile(ld_lin, 1);
+    }
     if (ld_k >= Ktot) {
       ld_k = 0;
       const int nl = ld_lin + G;
-      if (nl < tiles && p.tile_group[nl / tiles_n] >= 0) ld_lin = nl;
+      if (nl < tiles && (SEG || p.tile_group[nl / tiles_n] >= 0)) ld_lin = nl;
       set_load_tile(ld_lin, 0);
+    } else if (SEG && ld_k + 64 > ld_valid) {  // the last, partial step of a segment: rows past it re-read its last one
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int over = 2 * (wave + 8 * j) + (lane >> 5) - (ld_valid - 1 - ld_k);
+        if (over > 0) ld_off[4 + j] -= (uint32_t)over * (uint32_t)(2 * ld_ldw);
+      }
     }
   };
 
@@ -309,7 +344,7 @@ __global__ __launch_bounds__(512) void moe_gemm_nn_wide_kernel(MoeNnParams p, in
     }
   };
 
-  const int nk = Ktot / 64;
+  const int nk_all = Ktot / 64;
   Frag f0, f1;
 #pragma unroll
   for (int q = 0; q < 8; q++) issue_one(q, 0);
@@ -325,8 +360,18 @@ __global__ __launch_bounds__(512) void moe_gemm_nn_wide_kernel(MoeNnParams p, in
   int st = 0;  // stage of the current step
   for (int lin = first; lin < tiles; lin += G) {
     const int mt = lin / tiles_n;
-    if (p.tile_group[mt] < 0) break;
-    const int row0 = p.tile_row0[mt], rows = p.tile_rows[mt], n0 = (lin - mt * tiles_n) * 256;
+    const int n0 = (lin - mt * tiles_n) * 256;
+    int row0, rows, seg = 0, nk = nk_all;
+    if constexpr (SEG) {
+      seg = mt / seg_tiles;
+      row0 = (mt - seg * seg_tiles) * 256;
+      rows = min(256, p.M - row0);
+      nk = seg_steps(seg);
+    } else {
+      if (p.tile_group[mt] < 0) break;
+      row0 = p.tile_row0[mt];
+      rows = p.tile_rows[mt];
+    }
     for (int kt = 0; kt < nk; kt++) {
       const uint8_t* cur_sb = nw_lds + st * STAGE;
       const uint8_t* oth_sb = nw_lds + (st ^ 1) * STAGE;
@@ -343,6 +388,15 @@ __global__ __launch_bounds__(512) void moe_gemm_nn_wide_kernel(MoeNnParams p, in
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const int m = 128 * wm + 16 * i + r16;
+      if constexpr (SEG) {
+        float* cp = p.cf + ((int64_t)seg * p.M + row0 + m) * p.N + nb;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          if (m < rows && nb + 16 * j < p.N) *(f32x4*)(cp + 16 * j) = acc[i][j];
+          acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        continue;
+      }
       bf16_t* cp = p.c + (int64_t)(row0 + m) * p.ldc + nb;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
@@ -372,8 +426,11 @@ struct MoeTnParams {
   bf16_t* dw;
   int64_t lddw, dw_gstride;
   int N, K, E;
-  const int* cu;
+  const int* cu;  // null: one group (E = 1) of rows [0, rows)
+  int rows;
+  int n_store;    // output rows that exist (N counts the columns that dy holds; N unless dy is padded)
 };
+__device__ __forceinline__ int tn_row(const MoeTnParams& p, int e) { return p.cu ? p.cu[e] : e * p.rows; }
 
 template <int GB_ROWS>
 __global__ __launch_bounds__(256) void moe_gemm_tn_kernel(MoeTnParams p) {
@@ -381,7 +438,7 @@ __global__ __launch_bounds__(256) void moe_gemm_tn_kernel(MoeTnParams p) {
   __shared__ __attribute__((aligned(1024))) uint8_t yt[2][GB_TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t xt[2][GB_TILE];
   const int e = blockIdx.z;
-  const int lo = p.cu[e], hi = p.cu[e + 1];
+  const int lo = tn_row(p, e), hi = tn_row(p, e + 1);
   const int k0 = blockIdx.x * 128, n0 = blockIdx.y * 128;
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = threadIdx.x >> 6, wn = wave >> 1, wk = wave & 1;
@@ -443,7 +500,7 @@ __global__ __launch_bounds__(256) void moe_gemm_tn_kernel(MoeTnParams p) {
 #pragma unroll
   for (int f = 0; f < 4; f++) {
     const int n = n0 + 64 * wn + 16 * f + r16;
-    if (n >= p.N) continue;
+    if (n >= p.n_store) continue;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int k = k0 + 64 * wk + 16 * i + 4 * g;
@@ -493,8 +550,8 @@ __global__ __launch_bounds__(512) void moe_gemm_tn_wide_kernel(MoeTnParams p) {
   int iy[4], ix[4];                                    // row numbers of the next step to be issued
   auto tile_rows_of = [&](int lin, int& lo, int& hi) {
     const int e = lin / tpe;
-    lo = p.cu[e];
-    hi = p.cu[e + 1];
+    lo = tn_row(p, e);
+    hi = tn_row(p, e + 1);
   };
   auto set_load_tile = [&](int lin) {
     const int t = lin % tpe;
@@ -627,7 +684,7 @@ __global__ __launch_bounds__(512) void moe_gemm_tn_wide_kernel(MoeTnParams p) {
   for (int lin = first; lin < tiles; lin += G) {
     const int e = lin / tpe, t = lin - e * tpe;
     const int k0 = (t % tiles_k) << 8, n0 = (t / tiles_k) << 8;
-    const int nk = (p.cu[e + 1] - p.cu[e] + 63) >> 6;
+    const int nk = (tn_row(p, e + 1) - tn_row(p, e) + 63) >> 6;
     for (int kt = 0; kt < nk; kt++) {
       const uint8_t* cur_sb = tw_lds + st * STAGE;
       const uint8_t* oth_sb = tw_lds + (st ^ 1) * STAGE;
@@ -654,7 +711,7 @@ __global__ __launch_bounds__(512) void moe_gemm_tn_wide_kernel(MoeTnParams p) {
         pk.x = pack_bf16x2(acc[i][f][0], acc[i][f][1]);
         pk.y = pack_bf16x2(acc[i][f][2], acc[i][f][3]);
         acc[i][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (n < p.N && kb + 16 * i < p.K) *(uint2*)(cp + 16 * i) = pk;
+        if (n < p.n_store && kb + 16 * i < p.K) *(uint2*)(cp + 16 * i) = pk;
       }
     }
   }
@@ -790,6 +847,72 @@ __global__ __launch_bounds__(256) void router_topk_bwd_kernel(const void* __rest
 
 static inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+static int launch_gemm_tn(MoeTnParams p, int64_t num_experts, int64_t dy_rows, int64_t x_rows, hipStream_t stream) {
+  const int64_t N = p.N, K = p.K, gy = (N + 127) / 128;
+  // dy_rows / x_rows = rows addressable in dy / x: the wide kernel's 32-bit offsets must reach them
+  const int64_t lim = (int64_t)1 << 32;
+  const int64_t tiles = num_experts * ((K + 255) / 256) * ((N + 255) / 256);
+  if (N >= 256 && K >= 256 && dy_rows > 0 && x_rows > 0 && (dy_rows * p.lddy + N) * 2 < lim &&
+      (x_rows * p.ldx + K) * 2 < lim && tiles <= (1 << 30)) {
+    constexpr int LDS = 2 * 2 * 64 * 512;
+    static DeviceOnce once;
+    const int dev = once.slot();
+    if (once.need(dev)) {
+      if (hipFuncSetAttribute((const void*)moe_gemm_tn_wide_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) !=
+          hipSuccess) {
+        (void)hipGetLastError();
+        return VX_ERR_LAUNCH;
+      }
+      once.mark(dev);
+    }
+    const unsigned grid = (unsigned)(tiles >= 256 ? 256 : (tiles + 7) / 8 * 8);
+    moe_gemm_tn_wide_kernel<<<grid, 512, LDS, stream>>>(p);
+  } else {
+    moe_gemm_tn_kernel<TN_ROWS><<<dim3((unsigned)((K + 127) / 128), (unsigned)gy, (unsigned)num_experts), 256, 0, stream>>>(p);
+  }
+  return launch_status();
+}
+
+// One dense product over segments of the contraction (gemm_seg.h)
+int launch_gemm_nn_segments(const bf16_t* a, int64_t lda, const bf16_t* w, int64_t ldw, float* out, int64_t M, int64_t N,
+                            int64_t cols, int seg_cols, hipStream_t stream) {
+  const int64_t lim = (int64_t)1 << 32;
+  if (M <= 0 || N < 8 || N % 8 || lda % 8 || ldw % 8 || !al16(a) || !al16(w) || !al16(out) || seg_cols % 64 || cols <= 0)
+    return VX_ERR_UNSUPPORTED;
+  if ((M * lda + seg_cols) * 2 >= lim || (64 * ldw + N) * 2 >= lim || M > 0x7fffffff || N > 0x7fffffff || cols > 0x7fffffff) return VX_ERR_UNSUPPORTED;
+  const int64_t tm = (M + 255) / 256 * ((cols + seg_cols - 1) / seg_cols), tn = (N + 255) / 256, tiles = tm * tn;
+  if (tiles > (1 << 30)) return VX_ERR_UNSUPPORTED;
+  MoeNnParams p = {};
+  p.a[0] = a; p.lda[0] = lda; p.w[0] = w; p.ldw[0] = ldw; p.w_gstride[0] = seg_cols * ldw;
+  p.N = (int)N;
+  p.cf = out; p.M = (int)M; p.seg_cols = seg_cols; p.cols = (int)cols;
+  constexpr int LDS = 2 * 2 * 256 * 64 * 2;
+  static DeviceOnce once;
+  const int dev = once.slot();
+  if (once.need(dev)) {
+    if (hipFuncSetAttribute((const void*)moe_gemm_nn_wide_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) !=
+        hipSuccess) {
+      (void)hipGetLastError();
+      return VX_ERR_LAUNCH;
+    }
+    once.mark(dev);
+  }
+  const unsigned grid = (unsigned)(tiles >= 256 ? 256 : (tiles + 7) / 8 * 8);
+  moe_gemm_nn_wide_kernel<true><<<grid, 512, LDS, stream>>>(p, (int)tm, (int)tn);
+  return launch_status();
+}
+
+int launch_gemm_tn_rows(const bf16_t* dy, int64_t lddy, const bf16_t* x, int64_t ldx, bf16_t* dw, int64_t lddw, int64_t rows,
+                        int64_t N, int64_t n_store, int64_t K, hipStream_t stream) {
+  if (rows <= 0 || N % 8 || K % 8 || lddy % 8 || ldx % 8 || lddw % 4 || !al16(dy) || !al16(x) || ((uintptr_t)dw & 7))
+    return VX_ERR_UNSUPPORTED;
+  if ((N + 127) / 128 > 65535 || rows > 0x7fffffff || N > 0x7fffffff || K > 0x7fffffff) return VX_ERR_UNSUPPORTED;
+  MoeTnParams p = {};
+  p.dy = dy; p.lddy = lddy; p.x = x; p.ldx = ldx; p.dw = dw; p.lddw = lddw;
+  p.N = (int)N; p.K = (int)K; p.E = 1; p.rows = (int)rows; p.n_store = (int)n_store;
+  return launch_gemm_tn(p, 1, rows, rows, stream);
+}
+
 }  // namespace vx
 
 using namespace vx;
@@ -831,7 +954,7 @@ int vx_moe_gemm_nn(const void* a, int64_t lda, const int* a_src, const void* w, 
     static DeviceOnce once;
     const int dev = once.slot();
     if (once.need(dev)) {
-      if (hipFuncSetAttribute((const void*)moe_gemm_nn_wide_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) !=
+      if (hipFuncSetAttribute((const void*)moe_gemm_nn_wide_kernel<false>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) !=
           hipSuccess) {
         (void)hipGetLastError();
         return VX_ERR_LAUNCH;
@@ -839,7 +962,7 @@ int vx_moe_gemm_nn(const void* a, int64_t lda, const int* a_src, const void* w, 
       once.mark(dev);
     }
     const unsigned grid = (unsigned)(tiles >= 256 ? 256 : (tiles + 7) / 8 * 8);
-    moe_gemm_nn_wide_kernel<<<grid, 512, LDS, stream>>>(p, (int)max_tiles, (int)tn);
+    moe_gemm_nn_wide_kernel<false><<<grid, 512, LDS, stream>>>(p, (int)max_tiles, (int)tn);
     return launch_status();
   }
   moe_gemm_nn_kernel<NN_ROWS><<<dim3((unsigned)((N + 127) / 128), (unsigned)max_tiles), 256, 0, stream>>>(p);
@@ -895,28 +1018,8 @@ int vx_moe_gemm_tn(const void* dy, int64_t lddy, const int* dy_src, const void* 
   p.x = (const bf16_t*)x; p.ldx = ldx; p.x_src = x_src;
   p.dw = (bf16_t*)dw; p.lddw = lddw; p.dw_gstride = dw_gstride;
   p.N = (int)N; p.K = (int)K; p.E = (int)num_experts; p.cu = cu;
-  // dy_rows / x_rows = rows addressable in dy / x: the wide kernel's 32-bit offsets must reach them
-  const int64_t lim = (int64_t)1 << 32;
-  const int64_t tiles = num_experts * ((K + 255) / 256) * ((N + 255) / 256);
-  if (N >= 256 && K >= 256 && dy_rows > 0 && x_rows > 0 && (dy_rows * lddy + N) * 2 < lim &&
-      (x_rows * ldx + K) * 2 < lim && tiles <= (1 << 30)) {
-    constexpr int LDS = 2 * 2 * 64 * 512;
-    static DeviceOnce once;
-    const int dev = once.slot();
-    if (once.need(dev)) {
-      if (hipFuncSetAttribute((const void*)moe_gemm_tn_wide_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) !=
-          hipSuccess) {
-        (void)hipGetLastError();
-        return VX_ERR_LAUNCH;
-      }
-      once.mark(dev);
-    }
-    const unsigned grid = (unsigned)(tiles >= 256 ? 256 : (tiles + 7) / 8 * 8);
-    moe_gemm_tn_wide_kernel<<<grid, 512, LDS, stream>>>(p);
-  } else {
-    moe_gemm_tn_kernel<TN_ROWS><<<dim3((unsigned)((K + 127) / 128), (unsigned)gy, (unsigned)num_experts), 256, 0, stream>>>(p);
-  }
-  return launch_status();
+  p.n_store = (int)N;
+  return launch_gemm_tn(p, num_experts, dy_rows, x_rows, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,280 @@
+// Log-probabilities of given tokens straight from the hidden states and the output projection, and their gradients,
+// without logits in memory (mathematics and roundings: vocab_logprob.h). Beside vx_logprobs, which wants the
+// [T, V] logits (vexact/batch_invariant_ops/standalone_logprobs.py:28-55).
+//   forward : GEMM with the row statistics as its epilogue -> one (max, sum) per row and 256 columns -> fold per row
+//   backward: per piece of the vocabulary, GEMM with the derivative as its epilogue into a bf16 piece [T, piece], then
+//             d W rows of the piece = piece^T h, and fp32 partial sums of d h per segment of 8192 columns, folded in
+//             ascending order. The segments are at absolute positions, so the bits do not depend on the piece width.
+#include "gemm_core.h"
+#include "gemm_seg.h"
+#include "gemm_wide.h"
+#include "vocab_logprob.h"
+
+namespace vx {
+
+constexpr int VL_BM = 64, VL_BN = 256, VL_BK = 64;
+constexpr int VL_RB = VL_BK * 2 + 16;  // LDS row pitch: 16 bytes on, so that the rows of a fragment read hit distinct banks
+constexpr int VL_SEG = 8192;           // columns per partial sum of d h
+
+// The general kernel: any H that is a multiple of 8, any number of rows. 64 rows x 256 columns per workgroup, one
+// 64-column strip per wavefront, operands through registers into one of two LDS buffers.
+template <int EPI>
+__global__ __launch_bounds__(256) void vocab_gemm_kernel(GemmParams p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lx[2][VL_BM * VL_RB];
+  __shared__ __attribute__((aligned(16))) uint8_t lw[2][VL_BN * VL_RB];
+  __shared__ float2 strips[4][VL_BM];
+  const int row0 = blockIdx.y * VL_BM, n0 = blockIdx.x * VL_BN;
+  const int rows = min(VL_BM, p.M - row0), K = p.K;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r16 = lane & 15, g = lane >> 4;
+
+  // piece q = tid + 256 j: row q / 8, 16-byte piece q % 8 (the same for all j)
+  const int c8 = tid & 7;
+  const bf16_t* xrow[2];
+  const bf16_t* wrow[8];
+#pragma unroll
+  for (int j = 0; j < 2; j++) xrow[j] = p.x + (int64_t)(row0 + min((tid >> 3) + 32 * j, rows - 1)) * p.ldx;
+#pragma unroll
+  for (int j = 0; j < 8; j++) wrow[j] = p.w + (int64_t)min(n0 + (tid >> 3) + 32 * j, p.N - 1) * p.ldw;
+  uint4 gx[2], gw[8];
+  auto gload = [&](int k0) {
+    const int k = k0 + 8 * c8 < K ? k0 + 8 * c8 : 0;  // a piece past K re-reads the row's first one; zeroed in lstore
+#pragma unroll
+    for (int j = 0; j < 2; j++) gx[j] = ldg16_raw(xrow[j] + k);
+#pragma unroll
+    for (int j = 0; j < 8; j++) gw[j] = ldg16_raw(wrow[j] + k);
+  };
+  auto lstore = [&](int buf, int k0) {
+    const bool ok = k0 + 8 * c8 < K;
+#pragma unroll
+    for (int j = 0; j < 2; j++) *(uint4*)(&lx[buf][((tid >> 3) + 32 * j) * VL_RB + c8 * 16]) = mask16(gx[j], ok);
+#pragma unroll
+    for (int j = 0; j < 8; j++) *(uint4*)(&lw[buf][((tid >> 3) + 32 * j) * VL_RB + c8 * 16]) = mask16(gw[j], ok);
+  };
+
+  f32x4 acc[4][4];  // [row tile][weight fragment]
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int nk = (K + VL_BK - 1) / VL_BK;
+  gload(0);
+  lstore(0, 0);
+  __syncthreads();
+  for (int kt = 0; kt < nk; kt++) {
+    const int buf = kt & 1;
+    if (kt + 1 < nk) gload((kt + 1) * VL_BK);
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+      uint4 wf[4], xf[4];
+      // MFMA row rho of fragment j is weight row 16 (rho / 4) + 4 j + rho % 4 of the strip: a lane then holds 16
+      // consecutive columns
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        wf[j] = *(const uint4*)(&lw[buf][(64 * wave + 16 * (r16 >> 2) + 4 * j + (r16 & 3)) * VL_RB + (32 * ks + 8 * g) * 2]);
+#pragma unroll
+      for (int i = 0; i < 4; i++) xf[i] = *(const uint4*)(&lx[buf][(16 * i + r16) * VL_RB + (32 * ks + 8 * g) * 2]);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j] = mfma16(wf[j], xf[i], acc[i][j]);
+    }
+    if (kt + 1 < nk) lstore(buf ^ 1, (kt + 1) * VL_BK);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int m = 16 * i + r16;
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; e++) v[e] = acc[i][e >> 2][e & 3];
+    if constexpr (EPI == EPI_LSE) vocab_strip(p, v, row0 + m, m < rows, n0 + 64 * wave, &strips[wave][m]);
+    else vocab_dlogits(p, v, row0 + m, m < rows, n0 + 64 * wave);
+  }
+  if constexpr (EPI == EPI_LSE) {
+    __syncthreads();
+    if (tid < rows) vocab_fold_strips(p, &strips[0][tid], VL_BM, row0 + tid, n0);
+  }
+}
+
+// out = x[label] - lse, lse = M + log S over a row's tile statistics: 8 rows and 32 runs of tiles (s, s + 32, ...) per
+// workgroup, the runs then folded in ascending order.
+__global__ __launch_bounds__(256) void vocab_final_kernel(const float2* __restrict__ part, int64_t part_ld, int ntiles,
+                                                          const float* __restrict__ label_logit, const int64_t* __restrict__ labels,
+                                                          float* __restrict__ out, float* __restrict__ lse_out, int64_t T, int64_t V) {
+  __shared__ float2 red[32][8];
+  const int r = threadIdx.x & 7, s = threadIdx.x >> 3;
+  const int64_t row = (int64_t)blockIdx.x * 8 + r;
+  float m = -INFINITY, sum = 0.f;
+  if (row < T)
+    for (int t = s; t < ntiles; t += 32) {
+      const float2 v = part[(int64_t)t * part_ld + row];
+      vocab_fold(m, sum, v.x, v.y);
+    }
+  red[s][r] = make_float2(m, sum);
+  __syncthreads();
+  if (s != 0 || row >= T) return;
+  for (int i = 1; i < 32; i++) vocab_fold(m, sum, red[i][r].x, red[i][r].y);
+  const float ls = logf(sum);
+  if (lse_out) lse_out[row] = m + ls;
+  if (out) {
+    const int64_t lab = labels[row];
+    out[row] = lab >= 0 && lab < V ? (label_logit[row] - m) - ls : NAN;
+  }
+}
+
+// d h: acc (+)= the partial sums of a piece's segments, in ascending order; after the last piece rounded to bf16.
+// Four columns per thread.
+__global__ __launch_bounds__(256) void vocab_dh_kernel(const float* __restrict__ part, int nseg, int64_t stride, float* __restrict__ acc,
+                                                       int first, bf16_t* __restrict__ dh, int64_t ld, int64_t T, int H) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= T * H) return;
+  f32x4 a = first ? *(const f32x4*)(part + i) : *(const f32x4*)(acc + i);
+  for (int s = first ? 1 : 0; s < nseg; s++) a += *(const f32x4*)(part + s * stride + i);
+  if (dh) {
+    uint2 pk;
+    pk.x = pack_bf16x2(a[0], a[1]);
+    pk.y = pack_bf16x2(a[2], a[3]);
+    *(uint2*)(dh + i / H * ld + i % H) = pk;
+  } else {
+    *(f32x4*)(acc + i) = a;
+  }
+}
+
+// Logit products of the columns [0, N) of this launch's weights for all rows; row chunks keep the wide kernel's 32-bit
+// offsets in range.
+template <int EPI>
+static int launch_vocab_gemm(const GemmParams& p_in, int64_t T, hipStream_t stream) {
+  const int64_t lim = (int64_t)1 << 32;
+  int64_t chunk = T;
+  while ((chunk * p_in.ldx + p_in.K) * 2 >= lim || (chunk + 63) / 64 > 65535) chunk = (chunk / 2 + 255) / 256 * 256;
+  for (int64_t r0 = 0; r0 < T; r0 += chunk) {
+    GemmParams p = p_in;
+    p.M = (int)std::min(chunk, T - r0);
+    p.x += r0 * p.ldx;
+    p.labels += r0;
+    if (EPI == EPI_LSE) { p.lse_part += r0; p.label_logit += r0; }
+    else { p.lse += r0; p.d_out += r0; p.c += r0 * p.ldc; }
+    const int64_t tm = ((int64_t)p.M + WD_BM - 1) / WD_BM;
+    if (p.M > 64 && gemm_wide_launch_t<EPI, false>(p, tm, p.M, stream)) continue;
+    const dim3 grid((unsigned)(((int64_t)p.N + VL_BN - 1) / VL_BN), (unsigned)(((int64_t)p.M + VL_BM - 1) / VL_BM));
+    vocab_gemm_kernel<EPI><<<grid, 256, 0, stream>>>(p);
+  }
+  return launch_status();
+}
+
+static bool vocab_args_ok(const void* h, const void* w, int64_t T, int64_t V, int64_t H, int64_t ldh, int64_t ldw) {
+  return V <= 0x7fffff00 && H <= 0x7fffff00 && T <= 0x7fffff00 && gemm_fast_ok(h, w, H, ldh, ldw);
+}
+
+// columns of one launch: whole 256-column tiles, weight bytes within 32 bits
+static int64_t vocab_cols_limit(int64_t V, int64_t H, int64_t ldw) {
+  int64_t n = (V + 255) / 256 * 256;
+  while ((n * ldw + H) * 2 >= ((int64_t)1 << 32)) n = (n / 2 + 255) / 256 * 256;
+  return n;
+}
+
+static inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// The backward's piece: segments per piece so that the piece and its partial sums stay near 768 MB (the whole
+// vocabulary at once up to some hundred rows, one segment at a time from some ten thousand).
+struct VocabPlan {
+  int64_t segs, per, pieces, ld;  // segments of the vocabulary, of a piece; pieces; columns of the piece buffer
+  int64_t dlog_bytes, part_bytes, acc_bytes;
+};
+static VocabPlan vocab_plan(int64_t T, int64_t V, int64_t H) {
+  VocabPlan q;
+  q.segs = (V + VL_SEG - 1) / VL_SEG;
+  const int64_t seg_bytes = T * VL_SEG * 2 + T * H * 4;
+  const int64_t most = std::max<int64_t>(1, std::min(q.segs, ((int64_t)768 << 20) / std::max<int64_t>(1, seg_bytes)));
+  q.pieces = (q.segs + most - 1) / most;
+  q.per = (q.segs + q.pieces - 1) / q.pieces;
+  q.pieces = (q.segs + q.per - 1) / q.per;
+  q.ld = std::min(q.per * VL_SEG, (V + 63) / 64 * 64);
+  q.dlog_bytes = up256(T * q.ld * 2);
+  q.part_bytes = up256(q.per * T * H * 4);
+  q.acc_bytes = q.pieces > 1 ? up256(T * H * 4) : 0;
+  return q;
+}
+
+}  // namespace vx
+
+using namespace vx;
+
+extern "C" {
+
+int64_t vx_vocab_logprobs_workspace_bytes(int64_t T, int64_t V) {
+  if (T <= 0 || V <= 0) return 0;
+  return up256((V + 255) / 256 * T * 8) + up256(T * 4);
+}
+
+int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* labels, float* out, float* lse, int64_t T, int64_t V,
+                      int64_t H, int64_t ldh, int64_t ldw, float scale, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  if (!hidden || !weight || !labels || (!out && !lse) || T < 0 || V <= 0 || H <= 0) return VX_ERR_ARG;
+  if (!vocab_args_ok(hidden, weight, T, V, H, ldh, ldw)) return VX_ERR_UNSUPPORTED;
+  if (T == 0) return VX_OK;
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < vx_vocab_logprobs_workspace_bytes(T, V)) return VX_ERR_WORKSPACE;
+  const int64_t ntiles = (V + 255) / 256, step = vocab_cols_limit(V, H, ldw);
+  GemmParams p = {};
+  p.x = (const bf16_t*)hidden; p.ldx = ldh;
+  p.ldw = ldw; p.K = (int)H;
+  p.labels = labels; p.scale = scale; p.tokens = V;
+  p.lse_part = (float2*)workspace; p.part_ld = T;
+  p.label_logit = (float*)((uint8_t*)workspace + up256(ntiles * T * 8));
+  for (int64_t v0 = 0; v0 < V; v0 += step) {
+    p.w = (const bf16_t*)weight + v0 * ldw;
+    p.N = (int)std::min(step, V - v0);
+    p.vocab_base = (int)v0;
+    const int rc = launch_vocab_gemm<EPI_LSE>(p, T, stream);
+    if (rc != VX_OK) return rc;
+  }
+  vocab_final_kernel<<<(unsigned)((T + 7) / 8), 256, 0, stream>>>(p.lse_part, T, (int)ntiles, p.label_logit, labels, out, lse, T, V);
+  return launch_status();
+}
+
+int64_t vx_vocab_logprobs_bwd_workspace_bytes(int64_t T, int64_t V, int64_t H) {
+  if (T <= 0 || V <= 0 || H <= 0) return 0;
+  const VocabPlan q = vocab_plan(T, V, H);
+  return q.dlog_bytes + q.part_bytes + q.acc_bytes;
+}
+
+int vx_vocab_logprobs_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* lse, const float* d_out,
+                          void* d_hidden, void* d_weight, int64_t T, int64_t V, int64_t H, int64_t ldh, int64_t ldw, int64_t ld_dh,
+                          int64_t ld_dw, float scale, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  if (!hidden || !weight || !labels || !lse || !d_out || (!d_hidden && !d_weight) || T <= 0 || V <= 0 || H <= 0) return VX_ERR_ARG;
+  if (!vocab_args_ok(hidden, weight, T, V, H, ldh, ldw)) return VX_ERR_UNSUPPORTED;
+  if ((d_hidden && (ld_dh % 4 || ((uintptr_t)d_hidden & 7))) || (d_weight && (ld_dw % 4 || ((uintptr_t)d_weight & 7)))) return VX_ERR_UNSUPPORTED;
+  const VocabPlan q = vocab_plan(T, V, H);
+  const int64_t lim = (int64_t)1 << 32;
+  if ((T * q.ld + VL_SEG) * 2 >= lim || (q.per * VL_SEG * ldw + H) * 2 >= lim || (T * H / 4 + 255) / 256 > 0x7fffffff) return VX_ERR_UNSUPPORTED;
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < q.dlog_bytes + q.part_bytes + q.acc_bytes) return VX_ERR_WORKSPACE;
+  bf16_t* dlog = (bf16_t*)workspace;
+  float* part = (float*)((uint8_t*)workspace + q.dlog_bytes);
+  float* acc = (float*)((uint8_t*)workspace + q.dlog_bytes + q.part_bytes);
+  for (int64_t i = 0; i < q.pieces; i++) {
+    const int64_t v0 = i * q.per * VL_SEG, cols = std::min(q.per * VL_SEG, V - v0);
+    const bf16_t* w = (const bf16_t*)weight + v0 * ldw;
+    GemmParams p = {};
+    p.x = (const bf16_t*)hidden; p.ldx = ldh;
+    p.w = w; p.ldw = ldw; p.N = (int)cols; p.K = (int)H;
+    p.c = dlog; p.ldc = q.ld;
+    p.labels = labels; p.lse = lse; p.d_out = d_out; p.scale = scale; p.vocab_base = (int)v0; p.tokens = V;
+    int rc = launch_vocab_gemm<EPI_DLOGITS>(p, T, stream);
+    if (rc != VX_OK) return rc;
+    if (d_hidden) {
+      rc = launch_gemm_nn_segments(dlog, q.ld, w, ldw, part, T, H, cols, VL_SEG, stream);
+      if (rc != VX_OK) return rc;
+      const bool last = i + 1 == q.pieces;
+      vocab_dh_kernel<<<(unsigned)((T * H / 4 + 255) / 256), 256, 0, stream>>>(
+          part, (int)((cols + VL_SEG - 1) / VL_SEG), T * H, acc, i == 0, last ? (bf16_t*)d_hidden : nullptr, ld_dh, T, (int)H);
+    }
+    if (d_weight) {
+      rc = launch_gemm_tn_rows(dlog, q.ld, (const bf16_t*)hidden, ldh, (bf16_t*)d_weight + v0 * ld_dw, ld_dw, T,
+                               (cols + 63) / 64 * 64, cols, H, stream);
+      if (rc != VX_OK) return rc;
+    }
+  }
+  return launch_status();
+}
+
+}  // extern "C"

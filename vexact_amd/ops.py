@@ -265,6 +265,72 @@ def logprobs_backward(logits: torch.Tensor, labels: torch.Tensor, out: torch.Ten
     return d
 
 
+def _vocab_operands(hidden, weight, labels, temperature):
+    _need_gpu("hidden", hidden)
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError(f"vocab_logprobs: need hidden [T, H] and weight [V, H], got {tuple(hidden.shape)} and {tuple(weight.shape)}")
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise ValueError(f"vocab_logprobs supports bfloat16 only, got {hidden.dtype} and {weight.dtype}")
+    if labels.numel() != hidden.shape[0] or labels.dtype not in (torch.int32, torch.int64):
+        raise ValueError("vocab_logprobs: labels must be integers, one per row of hidden")
+    if weight.device != hidden.device or labels.device != hidden.device:
+        raise ValueError("vocab_logprobs: hidden, weight and labels must be on one device")
+    if not temperature > 0:
+        raise ValueError("vocab_logprobs: temperature must be positive")
+    if hidden.shape[1] % 8 or weight.shape[0] == 0:
+        raise ValueError(f"vocab_logprobs: H must be a multiple of 8 and V positive, got H = {hidden.shape[1]}, V = {weight.shape[0]}")
+    aligned = lambda t: t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0  # noqa: E731
+    x, w = (t if aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (hidden, weight))
+    return x, w, labels.reshape(-1).to(torch.int64).contiguous(), 1.0 / float(temperature)
+
+
+def vocab_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0):
+    """``(logprobs [T], lse [T])`` in fp32 of the tokens ``labels [T]`` under the logits ``hidden [T, H] @ weight [V, H].T /
+    temperature`` (bf16 operands, H a multiple of 8), which never reach memory. A label outside ``[0, V)`` gives NaN. A
+    row's bits depend on its own hidden state only; the logits are not rounded to bf16 as those of ``matmul`` are, so
+    they are not the bits of ``logprobs(matmul(...))``."""
+    x, w, lab, scale = _vocab_operands(hidden, weight, labels, temperature)
+    T, H = x.shape
+    out = _empty(T, dtype=torch.float32, device=x.device)
+    lse = _empty(T, dtype=torch.float32, device=x.device)
+    if T == 0:
+        return out, lse
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        ws = _workspace(lib.vx_vocab_logprobs_workspace_bytes(T, w.shape[0]), x.device)
+        _lib.check(
+            lib.vx_vocab_logprobs(x.data_ptr(), w.data_ptr(), lab.data_ptr(), out.data_ptr(), lse.data_ptr(), T, w.shape[0], H,
+                                  x.stride(0), w.stride(0), scale, ws.data_ptr(), ws.numel(), _stream()),
+            "vx_vocab_logprobs",
+        )
+    return out, lse
+
+
+def vocab_logprobs_backward(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor,
+                            d_out: torch.Tensor, temperature: float = 1.0, *, need_hidden: bool = True, need_weight: bool = True):
+    """``(d_hidden, d_weight)`` (bf16, None where not needed) of ``vocab_logprobs(hidden, weight, labels, temperature)[0]``
+    given its ``lse`` and the incoming ``d_out [T]``. The logits are computed again in pieces of the vocabulary; rows
+    without a valid label have no gradient."""
+    x, w, lab, scale = _vocab_operands(hidden, weight, labels, temperature)
+    (T, H), V = x.shape, w.shape[0]
+    d_x = _empty((T, H), dtype=x.dtype, device=x.device) if need_hidden else None
+    d_w = _empty((V, H), dtype=w.dtype, device=w.device) if need_weight else None
+    if lse.dtype != torch.float32 or lse.numel() != T or d_out.numel() != T:
+        raise ValueError("vocab_logprobs: lse (fp32, the forward's) and d_out must have one entry per row")
+    if T == 0 or not (need_hidden or need_weight):
+        return d_x, d_w.zero_() if need_weight else None
+    ls, g = lse.reshape(-1).contiguous(), d_out.reshape(-1).float().contiguous()
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        ws = _workspace(lib.vx_vocab_logprobs_bwd_workspace_bytes(T, V, H), x.device)
+        _lib.check(
+            lib.vx_vocab_logprobs_bwd(x.data_ptr(), w.data_ptr(), lab.data_ptr(), ls.data_ptr(), g.data_ptr(), _ptr(d_x), _ptr(d_w),
+                                      T, V, H, x.stride(0), w.stride(0), H, H, scale, ws.data_ptr(), ws.numel(), _stream()),
+            "vx_vocab_logprobs_bwd",
+        )
+    return d_x, d_w
+
+
 def sample_tokens(
     logits: torch.Tensor, temperature: float, top_k: Optional[int], top_p: float, seeds: torch.Tensor,
     positions: torch.Tensor, out: Optional[torch.Tensor] = None,
