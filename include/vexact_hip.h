@@ -363,6 +363,21 @@ int vx_moe_gemm_nn(const void* a, int64_t lda, const int* a_src, const void* w, 
 int vx_router_topk_bwd(const void* logits, const int64_t* idx, const void* d_weights, void* d_logits, int64_t T, int E,
                        int k, int64_t ld, int64_t ld_out, int logits_bf16, int weights_bf16, int renorm,
                        hipStream_t stream);
+/* Routing from softmax (sigmoid == 0) or sigmoid scores s of logits [T, E] (fp32 or bf16, row pitch ld): c = s + bias
+ * (bias [E] fp32, may be null; it takes part in the selection only); with n_groups > 1 a group of E / n_groups
+ * consecutive experts scores the sum of its best group_top (1 or 2) c, and experts outside the topk_groups best groups
+ * rank as -inf; idx [T, k] = the k largest c in descending order, weights [T, k] = scale * s / (renorm: sum of the
+ * selected s; all of them 0: weights 0). Ties go to the lower index, NaN ranks with -inf; scores and sums are held in
+ * 64 bits, so the selection is that of the exact scores. E <= 512, k <= 64, n_groups <= 64, topk_groups groups must
+ * hold at least k experts. vx_router_topk is the router of the reference's own block (softmax, no bias, no groups).
+ * The backward gives d_logits [T, E] (the logits' type) from idx (int64, distinct within a row; an index outside
+ * [0, E) selects nothing) and d_weights [T, k]. */
+int vx_router_grouped(const void* logits, const float* bias, void* weights, void* idx, int64_t T, int E, int k,
+                      int64_t ld, int sigmoid, int n_groups, int topk_groups, int group_top, int renorm, float scale,
+                      int logits_bf16, int weights_bf16, int idx_i64, hipStream_t stream);
+int vx_router_grouped_bwd(const void* logits, const int64_t* idx, const void* d_weights, void* d_logits, int64_t T,
+                          int E, int k, int64_t ld, int64_t ld_out, int sigmoid, int renorm, float scale,
+                          int logits_bf16, int weights_bf16, hipStream_t stream);
 /* The elementwise step of the same backward between the products (fused_moe.py:150-250: silu, its derivative, the
  * routing-weight gradient), one launch, bf16 with a rounding wherever one of the reference's tensor operations
  * rounds. For sorted row r, w = rw[flat[r]]: hw = silu(g) u w; d_rw[flat[r]] = sum_i (silu(g) u)(d_hw);

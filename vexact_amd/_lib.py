@@ -69,6 +69,8 @@ PROTOTYPES = {
     "vx_vocab_logprobs": (_I, [_P] * 5 + [_L] * 5 + [_F, _P, _L, _P]),
     "vx_vocab_logprobs_bwd_workspace_bytes": (_L, [_L, _L, _L]),
     "vx_vocab_logprobs_bwd": (_I, [_P] * 7 + [_L] * 7 + [_F, _P, _L, _P]),
+    "vx_router_grouped": (_I, [_P] * 4 + [_L, _I, _I, _L] + [_I] * 5 + [_F, _I, _I, _I, _P]),
+    "vx_router_grouped_bwd": (_I, [_P] * 4 + [_L, _I, _I, _L, _L, _I, _I, _F, _I, _I, _P]),
     "vx_router_topk_bwd": (_I, [_P, _P, _P, _P, _L, _I, _I, _L, _L, _I, _I, _I, _P]),
     "vx_moe_swiglu_bwd": (_I, [_P, _P, _P, _L, _L, _L, _P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _L, _P]),
     "vx_moe_gemm_tn": (_I, [_P, _L, _P, _P, _L, _P, _P, _L, _L, _L, _L, _P, _L, _L, _L, _P]),

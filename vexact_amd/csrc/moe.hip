@@ -92,16 +92,6 @@ __global__ __launch_bounds__(256) void router_topk_kernel(const void* __restrict
 // (equal values: lower index; -0 and +0 are equal), and the selected probability is recomputed from
 // the winner's value with the expression its owner used, so the outputs are bit-identical to the
 // kernel above.
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));   // lanes i ^ 1
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));   // lanes i ^ 2
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));  // half-row mirror
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));  // row mirror
-  const uint32_t a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16);
-  const uint32_t c = __builtin_amdgcn_readlane((int)v, 32), d = __builtin_amdgcn_readlane((int)v, 48);
-  return max(max(a, b), max(c, d));
-}
-
 template <int PER, bool OUT_BF16, bool IDX64>
 __global__ __launch_bounds__(256) void router_topk_bf16_kernel(const bf16_t* __restrict__ logits,
                                                                void* __restrict__ weights_out,

@@ -811,6 +811,82 @@ def router_topk_backward(logits: torch.Tensor, selected: torch.Tensor, d_weights
     return out
 
 
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _grouped_router_logits(logits, top_k, score):
+    _need_gpu("logits", logits)
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("router logits must be a [tokens, experts] tensor in float32 or bfloat16")
+    if score not in _SCORES:
+        raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
+    E = logits.shape[1]
+    if not 0 < E <= 512 or not 0 < top_k <= min(E, 64):
+        raise ValueError(f"need 1 to 512 experts and a top_k of at most 64 of them, got {E} and {top_k}")
+    return logits if logits.stride(1) == 1 and logits.stride(0) >= E else logits.contiguous()
+
+
+def router_topk_grouped(
+    logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None, n_groups: int = 1,
+    topk_groups: int = 1, group_top: int = 2, renorm: bool = True, scale: float = 1.0,
+    out_dtype: torch.dtype = torch.bfloat16, index_dtype: torch.dtype = torch.int64,
+):
+    """``(weights [T, k], experts [T, k])``: softmax or sigmoid scores, ``bias [E]`` (fp32) added for the selection only, the
+    ``topk_groups`` best of ``n_groups`` groups (by the sum of their best ``group_top`` biased scores), the ``top_k`` best
+    experts of those in descending order (ties: lower index), weights ``scale * score`` renormalised over the selected.
+    Scores are compared in 64 bits. ``router_topk`` is the router of the reference's own block."""
+    lg = _grouped_router_logits(logits, top_k, score)
+    T, E = lg.shape
+    if out_dtype not in (torch.float32, torch.bfloat16) or index_dtype not in (torch.int32, torch.int64):
+        raise ValueError("unsupported router output dtypes")
+    if not 1 <= n_groups <= 64 or E % n_groups or not 1 <= topk_groups <= n_groups or group_top not in (1, 2):
+        raise ValueError(f"need 1 to 64 equal groups of {E} experts, topk_groups of them and group_top 1 or 2, got {n_groups}, {topk_groups}, {group_top}")
+    if topk_groups * (E // n_groups) < top_k:
+        raise ValueError(f"{topk_groups} groups of {E // n_groups} experts do not hold top_k = {top_k}")
+    if bias is not None:
+        if bias.shape != (E,) or bias.dtype != torch.float32 or bias.device != lg.device:
+            raise ValueError("bias must be a float32 [experts] tensor on the logits' device")
+        bias = bias.contiguous()
+    w = _empty((T, top_k), dtype=out_dtype, device=lg.device)
+    idx = _empty((T, top_k), dtype=index_dtype, device=lg.device)
+    if T == 0:
+        return w, idx
+    with torch.cuda.device(lg.device):
+        _lib.check(
+            _lib.load().vx_router_grouped(
+                lg.data_ptr(), _ptr(bias), w.data_ptr(), idx.data_ptr(), T, E, top_k, lg.stride(0), _SCORES[score], n_groups,
+                topk_groups, group_top, int(renorm), float(scale), int(lg.dtype == torch.bfloat16),
+                int(out_dtype == torch.bfloat16), int(index_dtype == torch.int64), _stream(),
+            ),
+            "vx_router_grouped",
+        )
+    return w, idx
+
+
+def router_topk_grouped_backward(logits: torch.Tensor, selected: torch.Tensor, d_weights: torch.Tensor, *,
+                                 score: str = "softmax", renorm: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of ``router_topk_grouped(logits, k, ...)[0]`` with respect to ``logits [T, E]``, given the selected experts."""
+    lg = _grouped_router_logits(logits, selected.shape[-1], score)
+    T, E = lg.shape
+    k = selected.shape[-1]
+    if selected.shape != (T, k) or d_weights.shape != (T, k) or selected.device != lg.device or d_weights.device != lg.device:
+        raise ValueError("selected and d_weights must be [tokens, top_k] tensors on the logits' device")
+    dw = d_weights if d_weights.dtype in (torch.float32, torch.bfloat16) else d_weights.float()
+    dw, sel = dw.contiguous(), selected.to(torch.int64).contiguous()
+    out = _empty((T, E), dtype=lg.dtype, device=lg.device)
+    if T == 0:
+        return out
+    with torch.cuda.device(lg.device):
+        _lib.check(
+            _lib.load().vx_router_grouped_bwd(
+                lg.data_ptr(), sel.data_ptr(), dw.data_ptr(), out.data_ptr(), T, E, k, lg.stride(0), E, _SCORES[score],
+                int(renorm), float(scale), int(lg.dtype == torch.bfloat16), int(dw.dtype == torch.bfloat16), _stream(),
+            ),
+            "vx_router_grouped_bwd",
+        )
+    return out
+
+
 def moe_tile_rows(num_tokens: int, wide_ok: bool = True, packed_only: bool = False, packed: bool = False,
                   top_k: int = 8, num_experts: int = 128) -> int:
     """Rows per expert tile (any choice gives the same bits), chosen from the average number of rows an expert
