@@ -254,6 +254,26 @@ int vx_attention_typed(const void* q, const void* k, const void* v, void* out, f
                        int64_t max_pages, int page_size, float softmax_scale, int causal, int mode,
                        int max_seqlen_q, int dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
+/* Paged decode (at most one query token per sequence, as vx_attention mode 0) for a batch whose sequences share long
+ * prefixes: group g = the sequences group_offsets[g] .. group_offsets[g + 1] - 1 (ascending, int32 on the device), whose
+ * block tables name the same pages for their first prefix_lens[g] keys. Whole 256-key chunks of a shared prefix are
+ * computed once per group, everything else per sequence; same bits as vx_attention on the same tables. Sequences
+ * before the first or behind the last group, and groups of one, share nothing. A sequence without keys gets zeros;
+ * rows of out that belong to no sequence, or to one without a query token, are left as they were. max_prefix_len: an upper
+ * bound of prefix_lens that sizes the launch and the workspace (longer prefixes are shared up to it). bf16 (dtype 0) or
+ * fp16 (1), head sizes up to 256, Hq / Hkv <= 32, caches as for vx_attention. seq_order (may be null): the order in
+ * which the per-sequence part takes the sequences. The reference has no counterpart. */
+int64_t vx_shared_prefix_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t Hq, int64_t Hkv, int64_t Dv,
+                                         int64_t max_prefix_len);
+int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void* out, const int* seq_order,
+                               const int* cu_seqlens_q, const int* seqused_k, const int* block_table,
+                               const int* group_offsets, const int* prefix_lens, int64_t num_seqs, int64_t num_groups,
+                               int Hq, int Hkv, int Dk, int Dv, int64_t sqt, int64_t sqh, int64_t skb, int64_t skp,
+                               int64_t skh, int64_t svb, int64_t svp, int64_t svh, int64_t sot, int64_t soh,
+                               int64_t bt_stride, int64_t max_pages, int page_size, float softmax_scale,
+                               int64_t max_prefix_len, int dtype, void* workspace, int64_t workspace_bytes,
+                               hipStream_t stream);
+
 /* Backward of causal varlen attention on packed q [Tq, Hq, D], k / v [Tk, Hkv, D] (bf16, D = 64 or 128):
  * dq, dk, dv (bf16) from dout, the forward's out and lse. P and dS are rounded to bf16 before they
  * enter a matrix product, as in the reference; all sums run in an order fixed by the sequence's own

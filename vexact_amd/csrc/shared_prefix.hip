@@ -1,0 +1,75 @@
+// Entry point of decode attention over shared prefixes (shared_prefix.h), and the bf16 kernels for the head sizes they
+// are built for exactly.
+#include "shared_prefix.h"
+
+using namespace vx;
+
+extern "C" {
+
+static inline int64_t shared_items(int64_t num_seqs, int64_t num_groups, int64_t G) { return num_seqs * G / 16 + num_groups; }
+
+int64_t vx_shared_prefix_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t Hq, int64_t Hkv, int64_t Dv, int64_t max_prefix_len) {
+  if (num_seqs <= 0 || num_groups <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Dv <= 0 || max_prefix_len <= 0) return 0;
+  const int64_t img = ((Dv + 127) / 128 * 8 + 1) * 256;
+  return shared_items(num_seqs, num_groups, Hq / Hkv) * Hkv * (max_prefix_len / ATT_CHUNK) * img * 4;
+}
+
+int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void* out, const int* seq_order, const int* cu_seqlens_q,
+                               const int* seqused_k, const int* block_table, const int* group_offsets, const int* prefix_lens,
+                               int64_t num_seqs, int64_t num_groups, int Hq, int Hkv, int Dk, int Dv, int64_t sqt, int64_t sqh,
+                               int64_t skb, int64_t skp, int64_t skh, int64_t svb, int64_t svp, int64_t svh, int64_t sot, int64_t soh,
+                               int64_t bt_stride, int64_t max_pages, int page_size, float softmax_scale, int64_t max_prefix_len,
+                               int dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  if (!q || !k || !v || !out || !cu_seqlens_q || !seqused_k || !block_table) return VX_ERR_ARG;
+  if (num_groups > 0 && (!group_offsets || !prefix_lens)) return VX_ERR_ARG;
+  if (dtype != 0 && dtype != 1) return VX_ERR_UNSUPPORTED;
+  if (num_seqs < 0 || num_groups < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Dk <= 0 || Dv <= 0 || max_prefix_len < 0) return VX_ERR_ARG;
+  if (page_size <= 0 || max_pages <= 0) return VX_ERR_ARG;
+  if (Dk > 256 || Dv > 256 || Hq / Hkv > 32 || num_seqs > 65535 || Hq > 65535) return VX_ERR_UNSUPPORTED;
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 2 != 0) return VX_ERR_ARG;
+  if (num_seqs == 0) return VX_OK;
+  const int64_t max_kv = max_pages * (int64_t)page_size;
+  if (max_prefix_len > max_kv) max_prefix_len = max_kv;
+  const int64_t items = shared_items(num_seqs, num_groups, Hq / Hkv), chunks = max_prefix_len / ATT_CHUNK;
+  if (items > 65535 || chunks > 65535) return VX_ERR_UNSUPPORTED;
+  const int64_t need = vx_shared_prefix_workspace_bytes(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len);
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return VX_ERR_WORKSPACE;
+  // rows that 16-byte accesses cannot address go element by element
+  const bool elem = (sqt | sqh | skb | skp | skh | svb | svp | svh | sot | soh | (int64_t)Dk | (int64_t)Dv) % 8 != 0 ||
+                    ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 != 0;
+  AttnParams p = {};
+  p.dk = Dk; p.dv = Dv; p.elem = elem ? 1 : 0;
+  p.q = (const bf16_t*)q; p.sqt = sqt; p.sqh = sqh;
+  p.k = (const bf16_t*)k; p.skb = skb; p.skp = skp; p.skh = skh;
+  p.v = (const bf16_t*)v; p.svb = svb; p.svp = svp; p.svh = svh;
+  p.o = (bf16_t*)out; p.sot = sot; p.soh = soh;
+  p.cu_q = cu_seqlens_q; p.seqused_k = seqused_k;
+  p.block_table = block_table; p.bt_stride = bt_stride;
+  p.page_size = page_size;
+  p.page_shift = -1;
+  if ((page_size & (page_size - 1)) == 0) {
+    int s = 0;
+    while ((1 << s) < page_size) s++;
+    p.page_shift = s;
+  }
+  p.Hq = Hq; p.Hkv = Hkv; p.num_seqs = (int)num_seqs;
+  p.qk_scale = softmax_scale * 1.44269504f;
+  p.causal = 1;
+  p.seq_order = seq_order;
+  p.max_kv = (int)(max_kv > 0x7fffffff ? 0x7fffffff : max_kv);
+  SharedParams sp = {};
+  sp.group_off = group_offsets; sp.prefix_len = prefix_lens;
+  sp.num_groups = (int)num_groups;
+  sp.max_chunks = (int)chunks;
+  sp.part = (float*)workspace;
+  sp.img_floats = ((Dv + 127) / 128 * 8 + 1) * 256;
+  if (dtype == 0 && !elem) {
+    if (Dk == 128 && Dv == 128) return launch_shared_prefix<ElemBF16, 128, 128, false>(p, sp, items, stream);
+    if (Dk == 64 && Dv == 64) return launch_shared_prefix<ElemBF16, 64, 64, false>(p, sp, items, stream);
+  }
+  const int DVb = Dv > 128 ? 256 : (Dk > 64 || Dv > 64) ? 128 : 64;
+  const int DKb = (Dk > 128 || DVb == 256) ? 256 : DVb;
+  return dtype == 0 ? launch_shared_prefix_bf16_padded(p, sp, DKb, DVb, items, stream) : launch_shared_prefix_f16(p, sp, DKb, DVb, items, stream);
+}
+
+}  // extern "C"

@@ -689,6 +689,81 @@ def paged_attention(
     return o
 
 
+def shared_prefix_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    seqused_k: torch.Tensor,
+    page_table: torch.Tensor,
+    group_offsets: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    softmax_scale: float,
+    max_prefix_len: Optional[int] = None,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+    seq_order: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``paged_attention`` of a decode step (``max_seqlen_q == 1``) whose sequences share long prefixes, same bits: group
+    ``g`` holds the sequences ``group_offsets[g] .. group_offsets[g + 1] - 1`` (int32 ``[G + 1]``, ascending), whose block
+    tables name the same pages for the first ``prefix_lens[g]`` (int32 ``[G]``) keys; those are read once per group.
+    ``max_prefix_len`` bounds ``prefix_lens`` from above (default: the block table's width); it sizes the launch and the
+    workspace. A sequence without keys gets zeros. bf16 or fp16."""
+    _need_gpu("q", q)
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4 or page_table.dim() != 2:
+        raise ValueError("shared_prefix_attention: need q [tokens, heads, dim], caches [blocks, page, heads, dim] and a 2-D page table")
+    T, Hq, Dk = q.shape
+    Hkv, Dv, page = k_cache.shape[2], v_cache.shape[-1], k_cache.shape[1]
+    if k_cache.shape[-1] != Dk or v_cache.shape[:3] != k_cache.shape[:3] or Hq % Hkv:
+        raise ValueError(f"shared_prefix_attention: q {tuple(q.shape)} does not fit caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    o = out if out is not None else torch.empty((T, Hq, Dv), dtype=q.dtype, device=q.device)
+    if o.shape != (T, Hq, Dv):
+        raise ValueError(f"shared_prefix_attention: out must be {(T, Hq, Dv)}, got {tuple(o.shape)}")
+    dtype = _attn_dtype_code("shared_prefix_attention", q, k_cache, v_cache, o)
+    if dtype == 2:
+        raise ValueError("shared_prefix_attention supports bfloat16 and float16")
+    if Dk > 256 or Dv > 256 or Hq // Hkv > 32:
+        raise ValueError(f"head_dim must be <= 256 and at most 32 query heads may share a kv head, got {max(Dk, Dv)} and {Hq // Hkv}")
+    if q.stride(-1) != 1 or k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1 or o.stride(-1) != 1:
+        raise ValueError("q, k, v and out must be contiguous in the head dimension")
+    B, G = seqused_k.numel(), prefix_lens.numel()
+    if cu_seqlens_q.numel() != B + 1 or page_table.shape[0] != B or group_offsets.numel() != G + 1:
+        raise ValueError(f"shared_prefix_attention: {B} sequences and {G} groups need cu_seqlens_q [{B + 1}], a page table of {B} rows "
+                         f"and group_offsets [{G + 1}], got {cu_seqlens_q.numel()}, {page_table.shape[0]} and {group_offsets.numel()}")
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("seqused_k", seqused_k), ("page_table", page_table),
+                    ("group_offsets", group_offsets), ("prefix_lens", prefix_lens)):
+        if t.dtype != torch.int32 or t.device != q.device or t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise ValueError(f"{name} must be an int32 tensor on {q.device} with contiguous entries, got {t.dtype} on {t.device}")
+    if k_cache.device != q.device or v_cache.device != q.device or o.device != q.device:
+        raise ValueError("q, the caches and out must be on one device")
+    if seq_order is not None and (seq_order.dtype != torch.int32 or seq_order.numel() != B or not seq_order.is_contiguous()):
+        raise ValueError("seq_order must be a contiguous int32 permutation of the sequences")
+    if T == 0 or B == 0:
+        return o
+    width = page_table.shape[1] * page
+    longest = width if max_prefix_len is None else min(int(max_prefix_len), width)
+    if longest < 0:
+        raise ValueError("max_prefix_len must not be negative")
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        need = lib.vx_shared_prefix_workspace_bytes(B, G, Hq, Hkv, Dv, longest)
+        ws = workspace if workspace is not None and workspace.numel() * workspace.element_size() >= need else None
+        if ws is None and need > 0:
+            ws = _workspace(need, q.device)
+        _lib.check(
+            lib.vx_shared_prefix_attention(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), _ptr(seq_order), cu_seqlens_q.data_ptr(),
+                seqused_k.data_ptr(), page_table.data_ptr(), group_offsets.data_ptr(), prefix_lens.data_ptr(), B, G, Hq, Hkv, Dk, Dv,
+                q.stride(0), q.stride(1), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+                v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), o.stride(0), o.stride(1),
+                page_table.stride(0), page_table.shape[1], page, float(softmax_scale), longest, dtype,
+                _ptr(ws), ws.numel() * ws.element_size() if ws is not None else 0, _stream(),
+            ),
+            "vx_shared_prefix_attention",
+        )
+    return o
+
+
 def packed_attention(
     q: torch.Tensor,
     k: torch.Tensor,
