@@ -261,12 +261,12 @@ int vx_attention_typed(const void* q, const void* k, const void* v, void* out, f
  * before the first or behind the last group, and groups of one, share nothing. A sequence without keys gets zeros;
  * rows of out that belong to no sequence, or to one without a query token, are left as they were. max_prefix_len: an upper
  * bound of prefix_lens that sizes the launch and the workspace (longer prefixes are shared up to it). bf16 (dtype 0) or
- * fp16 (1), head sizes up to 256, Hq / Hkv <= 32, caches as for vx_attention. seq_order (may be null): the order in
- * which the per-sequence part takes the sequences. The reference has no counterpart. */
+ * fp16 (1), head sizes up to 256, Hq / Hkv <= 32, caches as for vx_attention. The workspace holds the chunk states
+ * (max_kv_len: max_pages * page_size). The reference has no counterpart. */
 int64_t vx_shared_prefix_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t Hq, int64_t Hkv, int64_t Dv,
-                                         int64_t max_prefix_len);
-int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void* out, const int* seq_order,
-                               const int* cu_seqlens_q, const int* seqused_k, const int* block_table,
+                                         int64_t max_prefix_len, int64_t max_kv_len);
+int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void* out, const int* cu_seqlens_q,
+                               const int* seqused_k, const int* block_table,
                                const int* group_offsets, const int* prefix_lens, int64_t num_seqs, int64_t num_groups,
                                int Hq, int Hkv, int Dk, int Dv, int64_t sqt, int64_t sqh, int64_t skb, int64_t skp,
                                int64_t skh, int64_t svb, int64_t svp, int64_t svh, int64_t sot, int64_t soh,

@@ -87,6 +87,8 @@ CASES = [  # groups, prefixes, tails, (Hq, Hkv), (Dk, Dv), page
     ([3], [600], [20], (4, 2), (192, 128), 16),
     ([3], [600], [700], (4, 2), (256, 256), 16),
     ([2], [520], [3], (24, 1), (256, 256), 16),
+    ([2, 3, 2, 2], [70, 130, 200, 63], [1, 60, 200], (8, 2), (128, 128), 16),  # less than a chunk shared, by whole blocks
+    ([6, 2], [447, 448], [1, 65, 1000], (16, 4), (64, 64), 16),
     ([3], [600], [20, 1], (6, 2), (36, 20), 16),  # rows that 16-byte accesses cannot address
     ([2, 2], [300, 256], [1], (4, 2), (64, 64), 1),  # pages of one key
 ]
@@ -109,12 +111,20 @@ def test_bits_and_value(groups, prefixes, tails, heads, dims, page, dtype):
 
 
 @gpu
+def test_long_tails_and_many_groups():
+    """Own chunks beyond one round of the workgroups that share them, and more groups than a wavefront has lanes."""
+    a = make([2, 1], [300, 100], [9000, 70, 4000], (4, 1), (128, 128), 16, seed=8)
+    assert_bitwise(ops.shared_prefix_attention(**a), paged(a, decode_kernel="split"))
+    a = make([1 + i % 3 for i in range(150)], [256 + 16 * (i % 40) for i in range(150)], [3, 90], (4, 2), (64, 64), 16, seed=9)
+    assert_bitwise(ops.shared_prefix_attention(**a), paged(a, decode_kernel="split"))
+    a = make([130], [700], [3, 90], (2, 1), (128, 128), 16, seed=10)  # more sequences than lanes
+    assert_bitwise(ops.shared_prefix_attention(**a), paged(a, decode_kernel="split"))
+
+
+@gpu
 def test_a_full_decode_batch():
     a = make([16] * 16, [1024 + 96 * i for i in range(16)], list(range(1, 600, 37)), (32, 4), (128, 128), 16, seed=3, head_major=True)
-    order = torch.argsort(a["seqused_k"], descending=True).int()
-    want = paged(a)
-    assert_bitwise(ops.shared_prefix_attention(**a), want)
-    assert_bitwise(ops.shared_prefix_attention(**a, seq_order=order), want)
+    assert_bitwise(ops.shared_prefix_attention(**a), paged(a))
 
 
 @gpu
@@ -195,7 +205,7 @@ def test_refusals_on_the_gpu():
     for change, what in (
         ({"q": a["q"].float()}, "one dtype"), ({"group_offsets": a["group_offsets"][:1]}, "groups need"), ({"seqused_k": a["seqused_k"].long()}, "int32"),
         ({"page_table": a["page_table"][:1]}, "groups need"), ({"prefix_lens": a["prefix_lens"].cpu()}, "int32 tensor on"),
-        ({"q": a["q"][:, :3]}, "does not fit"), ({"q": a["q"][..., :32]}, "does not fit"), ({"seq_order": torch.zeros(2).cuda()}, "seq_order"),
+        ({"q": a["q"][:, :3]}, "does not fit"), ({"q": a["q"][..., :32]}, "does not fit"),
         ({"max_prefix_len": -1}, "negative"), ({"out": torch.zeros(1, 4, 64, dtype=torch.bfloat16).cuda()}, "out must be"),
         ({"q": a["q"][:, :, ::2].repeat(1, 1, 2)[:, :, ::1].transpose(1, 2).contiguous().transpose(1, 2)}, "contiguous in the head"),
     ):
@@ -215,17 +225,18 @@ def test_c_abi_refusals():
         v = dict(q=p, k=p, v=p, o=p, cu=p, used=p, bt=p, go=p, pl=p, B=4, G=2, Hq=8, Hkv=2, Dk=128, Dv=128, pages=64, page=16, maxp=512, dt=0, ws=p, n=1 << 30)
         v.update(kw)
         return lib.vx_shared_prefix_attention(
-            v["q"], v["k"], v["v"], v["o"], None, v["cu"], v["used"], v["bt"], v["go"], v["pl"], v["B"], v["G"], v["Hq"], v["Hkv"], v["Dk"], v["Dv"],
+            v["q"], v["k"], v["v"], v["o"], v["cu"], v["used"], v["bt"], v["go"], v["pl"], v["B"], v["G"], v["Hq"], v["Hkv"], v["Dk"], v["Dv"],
             1024, 128, 4096, 256, 128, 4096, 256, 128, 1024, 128, v["pages"], v["pages"], v["page"], 1.0, v["maxp"], v["dt"], v["ws"], v["n"], None)
 
     assert call(B=0) == 0
     for bad in (dict(q=None), dict(k=None), dict(o=None), dict(cu=None), dict(used=None), dict(bt=None), dict(go=None), dict(pl=None), dict(B=-1),
                 dict(G=-1), dict(Hq=7), dict(Dk=0), dict(page=0), dict(pages=0), dict(maxp=-1), dict(q=p + 1)):
         assert call(**bad) == -1, bad
-    for bad in (dict(dt=2), dict(Dk=257), dict(Dv=300), dict(Hq=66, Hkv=2), dict(B=70000), dict(G=70000)):
+    for bad in (dict(dt=2), dict(Dk=257), dict(Dv=300), dict(Hq=66, Hkv=2), dict(B=70000), dict(G=1 << 28)):
         assert call(**bad) == -2, bad
     for bad in (dict(ws=None), dict(n=1000), dict(ws=p + 8)):
         assert call(**bad) == -3, bad
-    # items: 4 sequences x 4 heads / 16 + 2 groups; 2 kv heads, 2 chunks, 9 KB an image
-    assert lib.vx_shared_prefix_workspace_bytes(4, 2, 8, 2, 128, 512) == 3 * 2 * 2 * 9216
-    assert lib.vx_shared_prefix_workspace_bytes(4, 2, 8, 2, 128, 255) == 0
+    # 4 sequences x 4 heads / 16 + 2 groups = 3 tiles x 2 kv heads x 2 chunks of 16 rows, and 4 x 2 x 3 own chunks of 4 rows
+    assert lib.vx_shared_prefix_workspace_bytes(4, 2, 8, 2, 128, 512, 700) == (3 * 2 * 2 * 16 + 4 * 2 * 3 * 4) * 130 * 4
+    assert lib.vx_shared_prefix_workspace_bytes(4, 2, 8, 2, 128, 255, 256) == 4 * 2 * 4 * 130 * 4
+    assert lib.vx_shared_prefix_workspace_bytes(4, 2, 3, 1, 1, 0, 1) == 4 * 20 * 4  # rounded up to 16 bytes

@@ -46,8 +46,8 @@ PROTOTYPES = {
         _I,
         [_P] * 10 + [_L, _L, _I, _I, _I, _I] + [_L] * 12 + [_I, _F, _I, _I, _I, _I, _P, _L, _P],
     ),
-    "vx_shared_prefix_workspace_bytes": (_L, [_L] * 6),
-    "vx_shared_prefix_attention": (_I, [_P] * 10 + [_L, _L, _I, _I, _I, _I] + [_L] * 12 + [_I, _F, _L, _I, _P, _L, _P]),
+    "vx_shared_prefix_workspace_bytes": (_L, [_L] * 7),
+    "vx_shared_prefix_attention": (_I, [_P] * 9 + [_L, _L, _I, _I, _I, _I] + [_L] * 12 + [_I, _F, _L, _I, _P, _L, _P]),
     "vx_attention_bwd_workspace_bytes": (_L, [_L, _L]),
     "vx_attention_bwd": (_I, [_P] * 11 + [_L, _L, _L, _I, _I, _I, _P, _F, _I, _I, _P, _L, _P]),
     "vx_attention_bwd_typed": (_I, [_P] * 11 + [_L, _L, _L, _I, _I, _I, _I, _P, _F, _I, _I, _I, _P, _L, _P]),

@@ -499,58 +499,6 @@ __device__ __forceinline__ KVSource<KIND> make_source(const AttnParams& p, int s
   return s;
 }
 
-// Groups of sequences that share the pages of a prefix (shared_prefix.h): chunk states of the prefix are computed once
-// per tile of 16 query rows of a group and folded by the decode kernel in front of a sequence's own chunks.
-struct SharedParams {
-  const int* group_off;   // [num_groups + 1]: group g = sequences group_off[g] .. group_off[g + 1] - 1
-  const int* prefix_len;  // [num_groups]: keys whose pages the group's sequences share
-  int num_groups;
-  int max_chunks;         // chunks of a prefix that the workspace holds
-  float* part;            // chunk images [item][kv head][max_chunks], one 16-row tile each
-  int64_t img_floats;
-};
-struct SharedGroup {
-  int seq0, n;   // first sequence, how many
-  int item0;     // first 16-row tile (item) of the group
-  int chunks;    // whole chunks of keys that are computed once for the group
-  int src;       // a sequence of the group that holds all of them: its block table is read
-};
-// All 64 lanes call it. The shared keys end where the longest sequence of the group ends, whatever prefix_len says, so
-// that the block table that is read covers them.
-__device__ __forceinline__ SharedGroup shared_group(const AttnParams& p, const SharedParams& s, int g) {
-  const int lane = threadIdx.x & 63;
-  SharedGroup r;
-  r.seq0 = min(max(s.group_off[g], 0), p.num_seqs);
-  r.n = min(max(s.group_off[g + 1], r.seq0), p.num_seqs) - r.seq0;
-  r.item0 = (int)((int64_t)r.seq0 * (p.Hq / p.Hkv) / 16) + g;
-  int longest = 0;
-  r.src = r.seq0;
-  for (int b = 0; b < r.n; b += 64) {
-    const int len = b + lane < r.n ? min(p.seqused_k[r.seq0 + b + lane], p.max_kv) : 0;
-    int m = len;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
-    if (m > longest) {
-      longest = m;
-      r.src = r.seq0 + b + __builtin_ctzll(__ballot(len == m));
-    }
-  }
-  // a group of one shares nothing: its keys are read once either way
-  r.chunks = r.n < 2 ? 0 : min(min(max(s.prefix_len[g], 0), longest) / ATT_CHUNK, s.max_chunks);
-  return r;
-}
-// the last group g whose value(g) <= x, -1 if there is none; value() is increasing (all 64 lanes call it)
-template <typename F>
-__device__ __forceinline__ int last_group_at_most(int num_groups, int x, F value) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int b = 0; b < num_groups; b += 64) {
-    const int g = b + lane;
-    n += __popcll(__ballot(g < num_groups && value(min(g, num_groups - 1)) <= x));
-  }
-  return n - 1;
-}
-
 // ---------------------------------------------------------------------------------------
 // Decode: every sequence has at most one query token. grid = (Hkv, B, max_chunks), one
 // wavefront per block; query heads of the kv head are the MFMA columns (G <= 16 * QT).
@@ -626,10 +574,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void at
 // no HBM round trip for the chunk states and no second launch, but needs B * Hkv * NW wavefronts to
 // fill the machine.
 // ---------------------------------------------------------------------------------------
-// SHARED: the running state starts from the chunk states of the sequence's shared prefix (same fold, same order), the
-// wavefronts' chunks begin behind them, and a sequence without keys gets zeros.
-template <class ET, int DK, int DV, int QT, int KIND, int NW, bool PAD, bool SHARED = false>
-__device__ __forceinline__ void attn_decode_fused_body(const AttnParams& p, const SharedParams* sp = nullptr) {
+template <class ET, int DK, int DV, int QT, int KIND, int NW, bool PAD>
+__device__ __forceinline__ void attn_decode_fused_body(const AttnParams& p) {
   constexpr int NDV = (DV + 127) / 128, NI = QT * NDV * 8;
   constexpr int IMG4 = (NI + QT) * 64;   // float4 per chunk image
   constexpr int MAXE = 16 * QT * (DV / 4);  // owner elements: (head, 4 dims)
@@ -642,61 +588,19 @@ __device__ __forceinline__ void attn_decode_fused_body(const AttnParams& p, cons
   const int q0 = p.cu_q[seq];
   const int qlen = p.cu_q[seq + 1] - q0;
   const int kv_len = min(p.seqused_k[seq], p.max_kv);
-  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
-  const int G = p.Hq / p.Hkv;
-  const int64_t tok = q0 + qlen - 1;
-  const int nelem = G * (DV / 4);
-  if constexpr (SHARED) {
-    if (qlen <= 0) return;
-    if (kv_len <= 0) {
-      for (int e = tid; e < nelem; e += 64 * NW)
-        attn_st4<PAD>(p.o + tok * p.sot + (int64_t)(kvh * G + e / (DV / 4)) * p.soh, 4 * (e % (DV / 4)), make_uint2(0u, 0u),
-                      PAD ? p.dv : DV, PAD ? p.elem : 0);
-      return;
-    }
-  }
   if (qlen <= 0 || kv_len <= 0) return;  // uniform over the block
   if (p.single_mode == 1 && qlen != 1) return;  // inside a general launch: the general kernel takes these
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = tid >> 6;
+  const int G = p.Hq / p.Hkv;
+  const int64_t tok = q0 + qlen - 1;
   const int pos = kv_len - 1;
   const int nch = (kv_len + ATT_CHUNK - 1) / ATT_CHUNK;
-  int first_chunk = 0;
+  const int nelem = G * (DV / 4);
 
-  if constexpr (SHARED) {
-    constexpr int IMG = NDV * 8 * 64;  // float4 of a 16-row tile's accumulators; 64 of (m, l) behind them
-    const int gi = last_group_at_most(sp->num_groups, seq, [&](int i) { return sp->group_off[i]; });
-    SharedGroup sg = {0, 0, 0, 0, 0};
-    if (gi >= 0) sg = shared_group(p, *sp, gi);
-    if (seq >= sg.seq0 + sg.n) sg.chunks = 0;  // behind the last group
-    first_chunk = sg.chunks;
-    for (int e = tid; e < nelem; e += 64 * NW) {
-      const int hl = e / (DV / 4), d = 4 * (e % (DV / 4));
-      const int row = (seq - sg.seq0) * G + hl;
-      const int sl = ((d / 128) * 4 + (d % 32) / 8) * 2 + (d % 8) / 4;
-      const int ln = 16 * ((d % 128) / 32) + (row & 15);
-      const float4* ip = (const float4*)(sp->part + ((int64_t)(sg.item0 + (row >> 4)) * p.Hkv + kvh) * sp->max_chunks * sp->img_floats);
-      float4 A4 = make_float4(0.f, 0.f, 0.f, 0.f);
-      float M = -INFINITY, L = 0.f;
-      for (int c = 0; c < sg.chunks; c++, ip += sp->img_floats / 4) {
-        const float4 ml = ip[IMG + (row & 15)];
-        const float4 a = ip[sl * 64 + ln];
-        float Mn, A, B;
-        fold_scales(M, ml.x, Mn, A, B);
-        L = fold_add(L, A, ml.y, B);
-        A4.x = fold_add(A4.x, A, a.x, B);
-        A4.y = fold_add(A4.y, A, a.y, B);
-        A4.z = fold_add(A4.z, A, a.z, B);
-        A4.w = fold_add(A4.w, A, a.w, B);
-        M = Mn;
-      }
-      racc[e] = A4;
-      rml[e] = make_float2(M, L);
-    }
-  } else {
-    for (int e = tid; e < nelem; e += 64 * NW) {
-      racc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-      rml[e] = make_float2(-INFINITY, 0.f);
-    }
+  for (int e = tid; e < nelem; e += 64 * NW) {
+    racc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    rml[e] = make_float2(-INFINITY, 0.f);
   }
 
   AttnWave<ET, DK, DV, QT, PAD> w;
@@ -710,7 +614,7 @@ __device__ __forceinline__ void attn_decode_fused_body(const AttnParams& p, cons
   }
   const KVSource<KIND> src = make_source<KIND>(p, seq, kvh, 0, kv_len);
 
-  for (int c0 = first_chunk; c0 < nch; c0 += NW) {
+  for (int c0 = 0; c0 < nch; c0 += NW) {
     const int c = c0 + wave;
     if (c < nch) w.run_chunk(src, c * ATT_CHUNK, min(c * ATT_CHUNK + ATT_CHUNK, kv_len), kv_len, p.qk_scale);
     __syncthreads();  // the previous round's fold has finished reading the images

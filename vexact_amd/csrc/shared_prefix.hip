@@ -1,20 +1,26 @@
-// Entry point of decode attention over shared prefixes (shared_prefix.h), and the bf16 kernels for the head sizes they
-// are built for exactly.
+// Entry point of decode attention over shared prefixes (shared_prefix.h), and the kernels for the head sizes they are
+// built for exactly.
 #include "shared_prefix.h"
 
 using namespace vx;
 
 extern "C" {
 
-static inline int64_t shared_items(int64_t num_seqs, int64_t num_groups, int64_t G) { return num_seqs * G / 16 + num_groups; }
+// 16-row tiles of all groups, at most
+static inline int64_t shared_tiles(int64_t num_seqs, int64_t num_groups, int64_t G) { return num_seqs * G / 16 + num_groups; }
 
-int64_t vx_shared_prefix_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t Hq, int64_t Hkv, int64_t Dv, int64_t max_prefix_len) {
-  if (num_seqs <= 0 || num_groups <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Dv <= 0 || max_prefix_len <= 0) return 0;
-  const int64_t img = ((Dv + 127) / 128 * 8 + 1) * 256;
-  return shared_items(num_seqs, num_groups, Hq / Hkv) * Hkv * (max_prefix_len / ATT_CHUNK) * img * 4;
+static int64_t shared_part_bytes(int64_t num_seqs, int64_t num_groups, int64_t Hq, int64_t Hkv, int64_t Dv, int64_t max_prefix_len) {
+  return shared_tiles(num_seqs, num_groups, Hq / Hkv) * Hkv * (max_prefix_len / ATT_CHUNK) * shared_image_floats(16, Dv) * 4;
 }
 
-int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void* out, const int* seq_order, const int* cu_seqlens_q,
+int64_t vx_shared_prefix_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t Hq, int64_t Hkv, int64_t Dv, int64_t max_prefix_len,
+                                         int64_t max_kv_len) {
+  if (num_seqs <= 0 || num_groups < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Dv <= 0 || max_prefix_len < 0 || max_kv_len <= 0) return 0;
+  return shared_part_bytes(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len) +
+         num_seqs * Hkv * ((max_kv_len + ATT_CHUNK - 1) / ATT_CHUNK) * shared_image_floats(Hq / Hkv, Dv) * 4;
+}
+
+int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void* out, const int* cu_seqlens_q,
                                const int* seqused_k, const int* block_table, const int* group_offsets, const int* prefix_lens,
                                int64_t num_seqs, int64_t num_groups, int Hq, int Hkv, int Dk, int Dv, int64_t sqt, int64_t sqh,
                                int64_t skb, int64_t skp, int64_t skh, int64_t svb, int64_t svp, int64_t svh, int64_t sot, int64_t soh,
@@ -30,10 +36,11 @@ int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void
   if (num_seqs == 0) return VX_OK;
   const int64_t max_kv = max_pages * (int64_t)page_size;
   if (max_prefix_len > max_kv) max_prefix_len = max_kv;
-  const int64_t items = shared_items(num_seqs, num_groups, Hq / Hkv), chunks = max_prefix_len / ATT_CHUNK;
-  if (items > 65535 || chunks > 65535) return VX_ERR_UNSUPPORTED;
-  const int64_t need = vx_shared_prefix_workspace_bytes(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len);
-  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return VX_ERR_WORKSPACE;
+  const int64_t shared_bytes = shared_part_bytes(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len);
+  const int64_t need = vx_shared_prefix_workspace_bytes(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len, max_kv);
+  if (num_groups > 0x7fffffff || max_kv > 0x7fffff00 || num_seqs * Hq > 0x7fffffff) return VX_ERR_UNSUPPORTED;
+  if (shared_tiles(num_seqs, num_groups, Hq / Hkv) * Hkv * (max_prefix_len / ATT_CHUNK + 8) > 0x7fffffff) return VX_ERR_UNSUPPORTED;  // workgroups
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) return VX_ERR_WORKSPACE;
   // rows that 16-byte accesses cannot address go element by element
   const bool elem = (sqt | sqh | skb | skp | skh | svb | svp | svh | sot | soh | (int64_t)Dk | (int64_t)Dv) % 8 != 0 ||
                     ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 != 0;
@@ -55,21 +62,25 @@ int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void
   p.Hq = Hq; p.Hkv = Hkv; p.num_seqs = (int)num_seqs;
   p.qk_scale = softmax_scale * 1.44269504f;
   p.causal = 1;
-  p.seq_order = seq_order;
-  p.max_kv = (int)(max_kv > 0x7fffffff ? 0x7fffffff : max_kv);
+  p.max_kv = (int)max_kv;
   SharedParams sp = {};
   sp.group_off = group_offsets; sp.prefix_len = prefix_lens;
   sp.num_groups = (int)num_groups;
-  sp.max_chunks = (int)chunks;
-  sp.part = (float*)workspace;
-  sp.img_floats = ((Dv + 127) / 128 * 8 + 1) * 256;
-  if (dtype == 0 && !elem) {
-    if (Dk == 128 && Dv == 128) return launch_shared_prefix<ElemBF16, 128, 128, false>(p, sp, items, stream);
-    if (Dk == 64 && Dv == 64) return launch_shared_prefix<ElemBF16, 64, 64, false>(p, sp, items, stream);
+  sp.max_chunks = (int)(max_prefix_len / ATT_CHUNK);
+  sp.shared_part = (float*)workspace;
+  sp.shared_floats = shared_image_floats(16, Dv);
+  sp.own_part = (float*)((uint8_t*)workspace + shared_bytes);
+  sp.own_floats = shared_image_floats(Hq / Hkv, Dv);
+  sp.max_own = (int)((max_kv + ATT_CHUNK - 1) / ATT_CHUNK);
+  if (!elem) {
+    if (Dk == 128 && Dv == 128)
+      return dtype == 0 ? launch_shared_prefix<ElemBF16, 128, 128, false>(p, sp, stream) : launch_shared_prefix<ElemF16, 128, 128, false>(p, sp, stream);
+    if (Dk == 64 && Dv == 64)
+      return dtype == 0 ? launch_shared_prefix<ElemBF16, 64, 64, false>(p, sp, stream) : launch_shared_prefix<ElemF16, 64, 64, false>(p, sp, stream);
   }
   const int DVb = Dv > 128 ? 256 : (Dk > 64 || Dv > 64) ? 128 : 64;
   const int DKb = (Dk > 128 || DVb == 256) ? 256 : DVb;
-  return dtype == 0 ? launch_shared_prefix_bf16_padded(p, sp, DKb, DVb, items, stream) : launch_shared_prefix_f16(p, sp, DKb, DVb, items, stream);
+  return dtype == 0 ? launch_shared_prefix_bf16_padded(p, sp, DKb, DVb, stream) : launch_shared_prefix_f16(p, sp, DKb, DVb, stream);
 }
 
 }  // extern "C"

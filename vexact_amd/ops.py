@@ -702,7 +702,6 @@ def shared_prefix_attention(
     max_prefix_len: Optional[int] = None,
     out: Optional[torch.Tensor] = None,
     workspace: Optional[torch.Tensor] = None,
-    seq_order: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """``paged_attention`` of a decode step (``max_seqlen_q == 1``) whose sequences share long prefixes, same bits: group
     ``g`` holds the sequences ``group_offsets[g] .. group_offsets[g + 1] - 1`` (int32 ``[G + 1]``, ascending), whose block
@@ -736,8 +735,6 @@ def shared_prefix_attention(
             raise ValueError(f"{name} must be an int32 tensor on {q.device} with contiguous entries, got {t.dtype} on {t.device}")
     if k_cache.device != q.device or v_cache.device != q.device or o.device != q.device:
         raise ValueError("q, the caches and out must be on one device")
-    if seq_order is not None and (seq_order.dtype != torch.int32 or seq_order.numel() != B or not seq_order.is_contiguous()):
-        raise ValueError("seq_order must be a contiguous int32 permutation of the sequences")
     if T == 0 or B == 0:
         return o
     width = page_table.shape[1] * page
@@ -746,18 +743,18 @@ def shared_prefix_attention(
         raise ValueError("max_prefix_len must not be negative")
     lib = _lib.load()
     with torch.cuda.device(q.device):
-        need = lib.vx_shared_prefix_workspace_bytes(B, G, Hq, Hkv, Dv, longest)
+        need = lib.vx_shared_prefix_workspace_bytes(B, G, Hq, Hkv, Dv, longest, width)
         ws = workspace if workspace is not None and workspace.numel() * workspace.element_size() >= need else None
-        if ws is None and need > 0:
+        if ws is None:
             ws = _workspace(need, q.device)
         _lib.check(
             lib.vx_shared_prefix_attention(
-                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), _ptr(seq_order), cu_seqlens_q.data_ptr(),
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), cu_seqlens_q.data_ptr(),
                 seqused_k.data_ptr(), page_table.data_ptr(), group_offsets.data_ptr(), prefix_lens.data_ptr(), B, G, Hq, Hkv, Dk, Dv,
                 q.stride(0), q.stride(1), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
                 v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), o.stride(0), o.stride(1),
                 page_table.stride(0), page_table.shape[1], page, float(softmax_scale), longest, dtype,
-                _ptr(ws), ws.numel() * ws.element_size() if ws is not None else 0, _stream(),
+                ws.data_ptr(), ws.numel() * ws.element_size(), _stream(),
             ),
             "vx_shared_prefix_attention",
         )
