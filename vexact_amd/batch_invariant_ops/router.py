@@ -26,11 +26,14 @@ class _GroupedRouterFunction(torch.autograd.Function):
         ctx.save_for_backward(logits, selected)
         ctx.call = (score, renorm, scale)
         ctx.mark_non_differentiable(selected)
+        ctx.set_materialize_grads(False)  # no zeros for the gradient that the selection does not have
         return weights, selected
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_weights, _):
+        if d_weights is None:
+            return (None,) * 10
         logits, selected = ctx.saved_tensors
         score, renorm, scale = ctx.call
         d_logits = ops.router_topk_grouped_backward(logits, selected, d_weights, score=score, renorm=renorm, scale=scale)

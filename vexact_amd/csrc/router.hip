@@ -84,26 +84,37 @@ __global__ __launch_bounds__(256) void router_grouped_kernel(RouterParams p) {
   }
   if (p.n_groups > 1) {
     __syncthreads();
-    // lane g: the score of group g, then how many groups come before it
+    // 64 >> gb lanes per group (2^gb >= n_groups) take every such element of it, their best two are merged pairwise: 8
+    // groups of 32 take 4 reads and 3 merges where one lane per group took 32 reads (64 tokens 10.1 -> XX us)
     const int size = p.E / p.n_groups;
+    int gb = 0;
+    while ((1 << gb) < p.n_groups) gb++;
+    const int lpg = 64 >> gb, grp = lane >> (6 - gb), part = lane & (lpg - 1);
     double a = -INFINITY, b = -INFINITY;
-    if (lane < p.n_groups)
-      for (int j = 0; j < size; j++) {
-        const double c = cs[wv][lane * size + j];
-        if (c > a) { b = a; a = c; }
-        else if (c > b) b = c;
+    if (grp < p.n_groups)
+      for (int j = part; j < size; j += lpg) {
+        const double c = cs[wv][grp * size + j];
+        b = fmax(b, fmin(a, c));
+        a = fmax(a, c);
       }
-    const double score = p.group_top == 2 && size > 1 ? a + b : a;
-    int before = 0;
-    for (int h = 0; h < p.n_groups; h++) {
-      const double o = __shfl(score, h, 64);
-      before += o > score || (o == score && h < lane);
+    for (int o = 1; o < lpg; o <<= 1) {
+      const double oa = __shfl_xor(a, o, 64), ob = __shfl_xor(b, o, 64);
+      b = fmax(fmin(a, oa), fmax(b, ob));
+      a = fmax(a, oa);
     }
-    const uint64_t kept = __ballot(lane < p.n_groups && before < p.topk_groups);
+    const double score = p.group_top == 2 && size > 1 ? a + b : a;
+    int before = 0;  // groups that come before this lane's
+    for (int h = 0; h < p.n_groups; h++) {
+      const uint64_t bits = __builtin_bit_cast(uint64_t, score);
+      const double o = __builtin_bit_cast(double, ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(bits >> 32), h * lpg) << 32) |
+                                                      (uint32_t)__builtin_amdgcn_readlane((int)bits, h * lpg));
+      before += o > score || (o == score && h < grp);
+    }
+    const uint64_t kept = __ballot(grp < p.n_groups && before < p.topk_groups);  // bits grp * lpg ..
 #pragma unroll
     for (int i = 0; i < PER; i++) {
       const int e = lane + 64 * i;
-      if (e < p.E && !((kept >> (e / size)) & 1)) key[i] = order_key(-INFINITY);
+      if (e < p.E && !((kept >> (e / size * lpg)) & 1)) key[i] = order_key(-INFINITY);
     }
   }
   for (int j = 0; j < p.k; j++) {
@@ -111,15 +122,20 @@ __global__ __launch_bounds__(256) void router_grouped_kernel(RouterParams p) {
 #pragma unroll
     for (int i = 0; i < PER; i++) hi = max(hi, (uint32_t)(key[i] >> 32));
     hi = wave_max_u32(hi);
-    uint32_t lo = 0;
+    // almost always one expert holds the largest upper half; only otherwise the lower halves decide
+    int holders = 0;
 #pragma unroll
-    for (int i = 0; i < PER; i++) lo = max(lo, (uint32_t)(key[i] >> 32) == hi ? (uint32_t)key[i] : 0u);
-    lo = wave_max_u32(lo);
-    const uint64_t best = ((uint64_t)hi << 32) | lo;
+    for (int i = 0; i < PER; i++) holders += __popcll(__ballot((uint32_t)(key[i] >> 32) == hi));
+    uint32_t lo = 0;
+    if (holders > 1) {
+#pragma unroll
+      for (int i = 0; i < PER; i++) lo = max(lo, (uint32_t)(key[i] >> 32) == hi ? (uint32_t)key[i] : 0u);
+      lo = wave_max_u32(lo);
+    }
     bool open = true;  // wave-uniform: the lowest index that holds it is the first lane of the first i
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-      const uint64_t who = open ? __ballot(key[i] == best) : 0;
+      const uint64_t who = open ? __ballot((uint32_t)(key[i] >> 32) == hi && (holders == 1 || (uint32_t)key[i] == lo)) : 0;
       if (who) {
         open = false;
         if (lane == __builtin_ctzll(who)) {
