@@ -50,6 +50,8 @@ struct GemmParams {
   int64_t tokens;         // the whole vocabulary
 };
 
+__device__ __forceinline__ void vocab_strip(const GemmParams& p, float (&v)[16], int row, bool live, int col0, float2* dst);  // vocab_logprob.h
+
 __device__ __forceinline__ float silu_f32(float g) { return g / (1.0f + expf(-g)); }
 
 // out = r16(r16(r16(silu(r16(g))) * r16(u)) * w)
@@ -238,6 +240,29 @@ __global__ __launch_bounds__(64 * NW) void gemm_stream_kernel(GemmParams p) {
 
   // lane holds C[row 16 i + r16][col n0 + 4 g + j], j = 0..3
   const int nc = n0 + 4 * g;
+  if constexpr (EPI == EPI_LSE) {
+    // the block's 64 columns are one strip: through LDS into the order of vocab_strip, 16 consecutive columns per lane
+    static_assert(NW == 4 && BM * 68 * 4 <= BM * RB, "a strip is 64 columns, and fits the staging buffer");
+    float* lg = (float*)xs;  // [BM][68]
+    __syncthreads();         // everyone is done with the staged activations
+#pragma unroll
+    for (int i = 0; i < MT; i++) *(f32x4*)(lg + (16 * i + r16) * 68 + 16 * wave + 4 * g) = acc[i];
+    __syncthreads();
+    if (wave < MT) {
+      const int m = 16 * wave + r16;
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const f32x4 q = *(const f32x4*)(lg + m * 68 + 16 * g + 4 * e);
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[4 * e + c] = q[c];
+      }
+      float2 st;
+      vocab_strip(p, v, row0 + m, m < rows, blockIdx.x * 64, &st);
+      if (g == 0 && m < rows) p.lse_part[(int64_t)((p.vocab_base >> 6) + blockIdx.x) * p.part_ld + row0 + m] = st;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < MT; i++) {
     const int m = 16 * i + r16;

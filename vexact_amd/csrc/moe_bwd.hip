@@ -847,6 +847,109 @@ __global__ __launch_bounds__(256) void router_topk_bwd_kernel(const void* __rest
 
 static inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// The segment form for few tiles: 64 x 64 outputs per workgroup, 4 wavefronts of 32 x 32, both operands directly to LDS into a
+// ring of four 16 KB stages of 64 contraction rows (three steps of loads in flight; two workgroups on a CU). Rows are 128
+// bytes in both tiles; 16-byte piece c of activation row r at c ^ (r / 2) % 8, and of weight row r at c ^ 2 f(r), f = bit 1
+// of r and bit 3 above it: the eight rows that a transposing read touches at a time then start at eight different 32-byte
+// slots. Same MFMA chain per output as the 256 x 256 kernel. 300 rows x 32003 tokens x 1024: 169 -> 54 us, where the wide
+// kernel has 32 tiles for 256 CUs; four times the L2 traffic makes it level near 64 of them.
+constexpr int NR_STAGES = 4, NR_STAGE = 2 * 64 * 128;
+__global__ __launch_bounds__(256) void gemm_nn_segments_ring_kernel(MoeNnParams p, int tiles_n) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NR_STAGES * NR_STAGE];
+  const int tiles_m = (p.M + 63) >> 6;
+  const int seg = blockIdx.x / (tiles_m * tiles_n), rem = blockIdx.x - seg * tiles_m * tiles_n;
+  const int row0 = rem / tiles_n * 64, n0 = rem % tiles_n * 64;
+  const int valid = min(p.seg_cols, p.cols - seg * p.seg_cols), nk = (valid + 63) >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
+  const bf16_t* a = p.a[0] + (int64_t)seg * p.seg_cols;
+  const bf16_t* w = p.w[0] + (int64_t)seg * p.w_gstride[0];
+  const int64_t ldw = p.ldw[0];
+  // load instruction q = wave + 4 t: rows [8 (q % 8), + 8) of the activation (t < 2) or weight tile
+  auto wswz = [](int r) { return (((r >> 1) & 1) | ((r >> 2) & 2)) << 1; };
+  uint32_t off[4];
+  int wcol[2];
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    const int R = 8 * ((wave + 4 * t) & 7) + (lane >> 3), slot = lane & 7;
+    if (t < 2) {
+      off[t] = (uint32_t)(((int64_t)min(row0 + R, p.M - 1) * p.lda[0] + 8 * (slot ^ nn_swz_x(R))) * 2);
+    } else {
+      wcol[t - 2] = min(n0 + 8 * (slot ^ wswz(R)), p.N - 8);  // columns past N re-read the last piece
+      off[t] = (uint32_t)(((int64_t)R * ldw + wcol[t - 2]) * 2);
+    }
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t)lds;
+  auto issue = [&](int step) {  // past the last step it is read again into a stage that nobody reads
+    const int s = min(step, nk - 1);
+    const uint32_t dst = lds0 + (step & (NR_STAGES - 1)) * NR_STAGE;
+    const bool ragged = 64 * s + 64 > valid;  // rows past the segment's last one re-read it
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      uint32_t o = off[t];
+      if (t >= 2 && ragged) {
+        const int R = 8 * ((wave + 4 * t) & 7) + (lane >> 3);
+        o = (uint32_t)(((int64_t)min(R, valid - 1 - 64 * s) * ldw + wcol[t - 2]) * 2);
+      }
+      lds_load16_sv(dst + (t < 2 ? 0 : 64 * 128) + ((wave + 4 * t) & 7) * 1024, o, t < 2 ? a + 64 * s : w + (int64_t)64 * s * ldw);
+    }
+  };
+  f32x4 acc[2][2];  // [activation tile][weight fragment]
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int xoff = (32 * wm + r16) * 128 + ((g ^ (r16 >> 1)) * 16);
+  const int wrow = 8 * g + (r16 >> 2);
+  int woff[2][2];
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+      woff[j][h] = 64 * 128 + (wrow + 4 * h) * 128 + (((4 * wn + 2 * j + ((r16 >> 1) & 1)) ^ wswz(wrow + 4 * h)) << 4) + 8 * (r16 & 1);
+#pragma unroll
+  for (int t = 0; t < NR_STAGES - 1; t++) issue(t);
+  for (int s = 0; s < nk; s++) {
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // 4 loads per step and wavefront: step s has landed
+    __syncthreads();                                  // for everyone, and everyone is done with step s - 1
+    issue(s + NR_STAGES - 1);
+    const uint8_t* sb = lds + (s & (NR_STAGES - 1)) * NR_STAGE;
+    uint4 xf[2][2], wf[2][2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) xf[ks][i] = *(const uint4*)(sb + (xoff ^ (64 * ks)) + i * 2048);
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(sb + woff[j][0] + ks * 32 * 128));
+        const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(sb + woff[j][1] + ks * 32 * 128));
+        const uint2 lo2 = __builtin_bit_cast(uint2, lo), hi2 = __builtin_bit_cast(uint2, hi);
+        wf[ks][j] = make_uint4(lo2.x, lo2.y, hi2.x, hi2.y);
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = mfma16(wf[ks][j], xf[ks][i], acc[i][j]);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the ring's last loads still target our LDS
+  // lane holds C[row0 + 32 wm + 16 i + r16][n0 + 32 wn + 16 j + 4 g + c]
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int m = row0 + 32 * wm + 16 * i + r16;
+    if (m >= p.M) continue;
+    float* cp = p.cf + ((int64_t)seg * p.M + m) * p.N;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int n = n0 + 32 * wn + 16 * j + 4 * g;
+      if (n < p.N) *(f32x4*)(cp + n) = acc[i][j];
+    }
+  }
+}
+
 static int launch_gemm_tn(MoeTnParams p, int64_t num_experts, int64_t dy_rows, int64_t x_rows, hipStream_t stream) {
   const int64_t N = p.N, K = p.K, gy = (N + 127) / 128;
   // dy_rows / x_rows = rows addressable in dy / x: the wide kernel's 32-bit offsets must reach them
@@ -886,6 +989,11 @@ int launch_gemm_nn_segments(const bf16_t* a, int64_t lda, const bf16_t* w, int64
   p.a[0] = a; p.lda[0] = lda; p.w[0] = w; p.ldw[0] = ldw; p.w_gstride[0] = seg_cols * ldw;
   p.N = (int)N;
   p.cf = out; p.M = (int)M; p.seg_cols = seg_cols; p.cols = (int)cols;
+  if (tiles < 64) {  // too few 256 x 256 tiles for the chip
+    const int64_t tn64 = (N + 63) / 64, wgs = (M + 63) / 64 * tn64 * ((cols + seg_cols - 1) / seg_cols);
+    gemm_nn_segments_ring_kernel<<<(unsigned)wgs, 256, 0, stream>>>(p, (int)tn64);
+    return launch_status();
+  }
   constexpr int LDS = 2 * 2 * 256 * 64 * 2;
   static DeviceOnce once;
   const int dev = once.slot();

@@ -9,8 +9,11 @@
 //
 // Launch 1: chunk states ("images") of the shared prefixes and, in the same grid behind them, of the sequences' own
 // chunks, so that tails of any length fill the chip while the last prefix chunks run. Launch 2: folds a sequence's
-// images in ascending order. With enough query rows in the batch a row block instead walks the chunks of its prefix one
-// after the other and folds them in registers, which leaves one image instead of one per chunk (attn_shared_walk_kernel).
+// images in ascending order. (A row block that walks its chunks one after the other and folds them in registers needs no
+// images of them, but its steps are a chain, and at 16 groups of 16 it leaves half of the CUs without one: level at 8192
+// query rows, 4 times slower for one group of 64 on 32768 keys.)
+// At a full decode batch both launches run at the rate of a large copy: what they move is the prefixes once (241 MB at 16
+// groups of 16 on prefixes about 7400, 32 / 4 heads), their images twice (2 x 131 MB) and the tails (300 MB): 143 + 37 us.
 #pragma once
 #include "attn_core.h"
 
@@ -29,8 +32,8 @@ struct SharedParams {
   int64_t own_floats;
   int max_own;
   int blocks;             // launch 1: row blocks per (chunk, kv head), workgroups of the shared part,
-  int walked;              // != 0: one folded image per tile of a prefix instead of one per chunk
-  int shared_wgs, splits;  // and workgroups that share the own chunks of one (sequence, kv head)
+  int shared_wgs, own_wgs;  // (multiples of 8), of the own part, chunks that a shared workgroup takes,
+  int cpw, splits;         // and workgroups that share the own chunks of one (sequence, kv head)
 };
 
 static inline int64_t shared_image_floats(int64_t rows, int64_t dv) { return (rows * ((dv + 3) / 4 * 4 + 2) + 3) / 4 * 4; }
@@ -106,16 +109,26 @@ __device__ __forceinline__ int shared_block(const AttnParams& p, const SharedPar
   return -1;
 }
 
-// Launch 1, shared part: workgroup -> (chunk, kv head, row block). Consecutive workgroups go round the eight XCDs, each with
-// an L2 of its own: chunk c goes to XCD c % 8, where all row blocks of a (chunk, kv head) follow each other, so the second
-// row block of a large group finds the chunk's keys in the L2.
-__device__ __forceinline__ void shared_place(int blocks, int Hkv, int& block, int& kvh, int& chunk) {
-  const int local = blockIdx.x >> 3;
-  block = local % blocks;
-  kvh = local / blocks % Hkv;
-  chunk = local / blocks / Hkv * 8 + (blockIdx.x & 7);
+// Launch 1 holds shared and own workgroups; returns the index within the kind, -1 - index for an own one. They alternate in
+// proportion, so that a CU runs one that waits for the matrix core beside one that waits for memory (16 groups of 16: 160 ->
+// 153 us); always eight consecutive ids, which go round the eight XCDs, are of one kind.
+__device__ __forceinline__ int shared_kind(const SharedParams& sp) {
+  const int grp = blockIdx.x >> 3;
+  const int64_t own = sp.own_wgs >> 3, all = own + (sp.shared_wgs >> 3);
+  const int before = (int)(grp * own / all), upto = (int)((grp + 1) * own / all);
+  return upto > before ? -1 - (before * 8 + (int)(blockIdx.x & 7)) : (grp - before) * 8 + (int)(blockIdx.x & 7);
 }
-static inline int64_t shared_wgs(int64_t blocks, int Hkv, int chunks) { return blocks * Hkv * ((chunks + 7) / 8 * 8); }
+
+// Shared workgroup -> (first chunk, kv head, row block). An XCD has an L2 of its own: chunk c belongs to XCD c % 8, where all
+// row blocks of a (chunk, kv head) follow each other, so the second row block of a large group finds the chunk's keys in
+// the L2. A workgroup takes cpw chunks, 8 apart.
+__device__ __forceinline__ void shared_place(const SharedParams& sp, int index, int Hkv, int& block, int& kvh, int& chunk) {
+  const int local = index >> 3;
+  block = local % sp.blocks;
+  kvh = local / sp.blocks % Hkv;
+  chunk = local / sp.blocks / Hkv * (8 * sp.cpw) + (index & 7);
+}
+static inline int64_t shared_wgs(int64_t blocks, int Hkv, int chunks, int cpw) { return blocks * Hkv * ((chunks + 8 * cpw - 1) / (8 * cpw) * 8); }
 
 // the state of one 16-row tile in the registers of AttnWave -> an image of `rows` rows (lane r16 = row `row`)
 template <class W>
@@ -137,14 +150,13 @@ __device__ __forceinline__ void shared_store(const W& w, int t, float* image, in
   if (g == 0) ((float2*)(image + (int64_t)4 * d4n * rows))[row] = make_float2(w.m[t], w.l[t]);
 }
 
-// Launch 1, own part, workgroups behind the shared ones: wavefront i of WAVES in workgroup (u, z) takes the own chunks
+// Launch 1, own part: wavefront i of WAVES in workgroup (u, z) takes the own chunks
 // z WAVES + i, + splits WAVES, ... of pair u = (sequence, kv head). A run of pairs goes to one XCD, so that the keys of the
 // partly shared chunk at a prefix's end come from its L2 for all but the first sequence of a group.
 template <class ET, int DK, int DV, int QT, int KIND, int WAVES, bool PAD>
-__device__ __forceinline__ void attn_own_chunks(const AttnParams& p, const SharedParams& sp) {
+__device__ __forceinline__ void attn_own_chunks(const AttnParams& p, const SharedParams& sp, int o) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, r16 = lane & 15;
-  const int o = blockIdx.x - sp.shared_wgs;  // shared_wgs is a multiple of 8
   const int per = ((int64_t)p.num_seqs * p.Hkv + 7) / 8;  // pairs of an XCD
   const int local = o >> 3, u = (o & 7) * per + local / sp.splits, z = local % sp.splits;
   if (local / sp.splits >= per || u >= p.num_seqs * p.Hkv) return;
@@ -180,12 +192,13 @@ __device__ __forceinline__ void attn_own_chunks(const AttnParams& p, const Share
 // Launch 1 for any head size: one wavefront per workgroup; a 16-row tile of a group and chunk, or an own chunk.
 template <class ET, int DK, int DV, int QT, int KIND, bool PAD>
 __global__ __launch_bounds__(64) void attn_shared_chunks_kernel(AttnParams p, SharedParams sp) {
-  if ((int)blockIdx.x >= sp.shared_wgs) {
-    attn_own_chunks<ET, DK, DV, QT, KIND, 1, PAD>(p, sp);
+  const int index = shared_kind(sp);
+  if (index < 0) {
+    attn_own_chunks<ET, DK, DV, QT, KIND, 1, PAD>(p, sp, -1 - index);
     return;
   }
   int block, kvh, chunk, place;
-  shared_place(sp.blocks, p.Hkv, block, kvh, chunk);
+  shared_place(sp, index, p.Hkv, block, kvh, chunk);
   const int G = p.Hq / p.Hkv;
   const int gi = shared_block(p, sp, block, 16, place);
   if (gi < 0) return;
@@ -215,11 +228,15 @@ template <int KIND>
 struct SharedLoader {
   KVSource<KIND> src;
   uint32_t lds0, koff[4], voff[4];
-  int wave, pg_cache, pg_base;  // SRC_FAST: page ids of this wavefront's tile for 64 blocks from pg_base, one per lane
+  int wave, c0, cstep;    // position i of the walk is block i % 4 of chunk c0 + cstep (i / 4)
+  int pg_cache, pg_base;  // SRC_FAST: page ids of this wavefront's tile for 64 positions from pg_base, one per lane
 
-  __device__ __forceinline__ void init(const AttnParams& p, int seq, int kvh, int keys, const uint8_t* lds, int wave_) {
+  __device__ __forceinline__ int key_at(int i) const { return (c0 + cstep * (i >> 2)) * ATT_CHUNK + (i & 3) * ATT_BLOCK + 16 * wave; }
+  __device__ __forceinline__ void init(const AttnParams& p, int seq, int kvh, int keys, const uint8_t* lds, int wave_, int c0_, int cstep_) {
     src = make_source<KIND>(p, seq, kvh, 0, keys);
     wave = wave_;
+    c0 = c0_;
+    cstep = cstep_;
     const int lane = threadIdx.x & 63;
     lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds + wave * 16 * 256;
     pg_cache = 0;
@@ -236,15 +253,15 @@ struct SharedLoader {
     return (const void*)(uintptr_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
                                     (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
   }
-  __device__ __forceinline__ void issue(int b, int stage) {  // block b of the prefix
-    const int key0 = b * ATT_BLOCK + 16 * wave;
+  __device__ __forceinline__ void issue(int i, int stage) {
+    const int key0 = key_at(i);
     const uint32_t dst = lds0 + stage * SPL_STAGE;
     if constexpr (KIND == SRC_FAST) {
-      if (b - pg_base >= 64 || b < pg_base) {  // wave-uniform
-        pg_base = b;
-        pg_cache = src.bt[min(key0 + (int)(threadIdx.x & 63) * ATT_BLOCK, src.last) >> src.shift];
+      if (i - pg_base >= 64) {  // wave-uniform
+        pg_base = i;
+        pg_cache = src.bt[min(key_at(i + (int)(threadIdx.x & 63)), src.last) >> src.shift];
       }
-      const int pg = __builtin_amdgcn_readlane(pg_cache, b - pg_base), off = key0 & (src.ps - 1);
+      const int pg = __builtin_amdgcn_readlane(pg_cache, i - pg_base), off = key0 & (src.ps - 1);
       const void* kt = uniform(src.kbase + (int64_t)pg * src.skb + (int64_t)off * src.skp);
       const void* vt = uniform(src.vbase + (int64_t)pg * src.svb + (int64_t)off * src.svp);
 #pragma unroll
@@ -338,14 +355,15 @@ __device__ __forceinline__ void shared_block_compute(const uint8_t* ks, int kb, 
 // bits). Every wavefront loads the 16 keys of one tile of the block. A chunk is read once per 64 TILES query rows.
 template <int TILES, int QT, int KIND>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_chunks_lds_kernel(AttnParams p, SharedParams sp) {
-  if ((int)blockIdx.x >= sp.shared_wgs) {
-    attn_own_chunks<ElemBF16, 128, 128, QT, KIND, 4, false>(p, sp);
+  const int index = shared_kind(sp);
+  if (index < 0) {
+    attn_own_chunks<ElemBF16, 128, 128, QT, KIND, 4, false>(p, sp, -1 - index);
     return;
   }
   constexpr int D = 128, KS = D / 32, RB = 64 * TILES;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * SPL_STAGE];
   int block, kvh, chunk, place;
-  shared_place(sp.blocks, p.Hkv, block, kvh, chunk);
+  shared_place(sp, index, p.Hkv, block, kvh, chunk);
   const int G = p.Hq / p.Hkv;
   const int gi = shared_block(p, sp, block, RB, place);
   if (gi < 0) return;
@@ -357,119 +375,51 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int keys = sg.chunks * ATT_CHUNK;  // every one of them exists
 
+  const int mine = min(sp.cpw, (sg.chunks - chunk + 7) >> 3), n = nb * mine;  // chunks, blocks of this workgroup
   SharedLoader<KIND> ld;
-  ld.init(p, sg.src, kvh, keys, lds, wave);
-  const int b0 = chunk * nb;
-  ld.issue(b0, 0);
-  ld.issue(b0 + 1, 1);
+  ld.init(p, sg.src, kvh, keys, lds, wave, chunk, 8);
+  ld.issue(0, 0);
+  ld.issue(1, 1);
 
   // ---- this wavefront's query tiles
   uint4 qf[TILES][KS];
   int qpos[TILES], qpos_min[TILES];
   shared_load_queries<TILES>(p, sg, kvh, row0 + 16 * wave * TILES, keys, qf, qpos, qpos_min);
-  float m[TILES], l[TILES];
-  f32x4 acc[TILES][8];
-#pragma unroll
-  for (int t = 0; t < TILES; t++) {
-    m[t] = -INFINITY;
-    l[t] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
   const bool any = row0 + 16 * wave * TILES < rows;  // wave-uniform: a wavefront without rows only loads
+  for (int c = 0; c < mine; c++) {
+    float m[TILES], l[TILES];
+    f32x4 acc[TILES][8];
 #pragma unroll
-  for (int b = 0; b < nb; b++) {
-    // 8 loads per block and wavefront, the youngest of which are those of block b + 1: at most 8 outstanding means that
-    // block b has landed
-    if (b + 1 < nb) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (any) shared_block_compute<TILES>(lds + (b & 1) * SPL_STAGE, chunk * ATT_CHUNK + b * ATT_BLOCK, p.qk_scale, qf, qpos, qpos_min, m, l, acc);
-    __syncthreads();  // everyone has read the stage
-    if (b + 2 < nb) ld.issue(b0 + b + 2, b & 1);
-  }
-
-  // lane (r16 = query row, g) holds dims 16 f + 4 g .. + 3 of fragment f
+    for (int t = 0; t < TILES; t++) {
+      m[t] = -INFINITY;
+      l[t] = 0.f;
 #pragma unroll
-  for (int t = 0; t < TILES; t++) {
-    const int lr = row0 + 16 * (wave * TILES + t);
-    if (lr + r16 >= rows) continue;
-    float* image = sp.shared_part + (((int64_t)(sg.tile0 + (lr >> 4)) * p.Hkv + kvh) * sp.max_chunks + chunk) * sp.shared_floats;
-#pragma unroll
-    for (int f = 0; f < 8; f++)
-      ((float4*)image)[(4 * f + g) * 16 + r16] = make_float4(acc[t][f][0], acc[t][f][1], acc[t][f][2], acc[t][f][3]);
-    if (g == 0) ((float2*)(image + D * 16))[r16] = make_float2(m[t], l[t]);
-  }
-}
-
-// Launch 1 for bf16 heads of 128 in large batches: a workgroup of 4 wavefronts (64 query rows) walks all shared chunks of its
-// group and folds them in registers: one image per tile in place of one per chunk. Four 32 KB stages keep three blocks of
-// loads in flight, one barrier per block. The row blocks 2 i and 2 i + 1 of a kv head go to one XCD, so that a group of 128
-// rows reads its keys from HBM once.
-constexpr int SPW_STAGES = 4;
-static inline int64_t walk_wgs(int64_t blocks, int Hkv) { return 16 * (((blocks + 1) / 2 * Hkv + 7) / 8); }
-template <int QT, int KIND>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_walk_kernel(AttnParams p, SharedParams sp) {
-  if ((int)blockIdx.x >= sp.shared_wgs) {
-    attn_own_chunks<ElemBF16, 128, 128, QT, KIND, 4, false>(p, sp);
-    return;
-  }
-  constexpr int D = 128, KS = D / 32, RB = 64;
-  extern __shared__ __attribute__((aligned(1024))) uint8_t sw_lds[];
-  const int local = blockIdx.x >> 3, v = (local >> 1) * 8 + (blockIdx.x & 7);
-  const int block = 2 * (v / p.Hkv) + (local & 1), kvh = v % p.Hkv;
-  int place;
-  const int gi = shared_block(p, sp, block, RB, place);
-  if (gi < 0) return;
-  const SharedGroup sg = shared_group(p, sp, gi);
-  const int rows = sg.n * (p.Hq / p.Hkv), row0 = place * RB;
-  if (sg.chunks == 0 || row0 >= rows) return;  // uniform over the block
-  const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int keys = sg.chunks * ATT_CHUNK, nblk = sg.chunks * (ATT_CHUNK / ATT_BLOCK);
-  SharedLoader<KIND> ld;
-  ld.init(p, sg.src, kvh, keys, sw_lds, wave);
-  uint4 qf[1][KS];
-  int qpos[1], qpos_min[1];
-  shared_load_queries<1>(p, sg, kvh, row0 + 16 * wave, keys, qf, qpos, qpos_min);
-#pragma unroll
-  for (int b = 0; b < SPW_STAGES - 1; b++) ld.issue(b, b);  // a chunk has four blocks: they exist
-  float M = -INFINITY, L = 0.f;
-  f32x4 ACC[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) ACC[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int b0 = 0; b0 < nblk; b0 += 4) {
-    float m[1] = {-INFINITY}, l[1] = {0.f};
-    f32x4 acc[1][8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) acc[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int b = b0 + i;
-      // 8 loads per block and wavefront, in order: all but the youngest two blocks' have landed
-      if (b + 2 < nblk) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-      else if (b + 1 < nblk) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();  // block b is there for everyone, and everyone is done with block b - 1
-      if (b + 3 < nblk) ld.issue(b + 3, (i + 3) & 3);
-      shared_block_compute<1>(sw_lds + i * SPL_STAGE, b * ATT_BLOCK, p.qk_scale, qf, qpos, qpos_min, m, l, acc);
+      for (int i = 0; i < 8; i++) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    float Mn, A, B;
-    fold_scales(M, m[0], Mn, A, B);
-    L = fold_add(L, A, l[0], B);
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+    for (int b = 0; b < nb; b++) {
+      const int i = c * nb + b;
+      // 8 loads per block and wavefront, the youngest of which are those of the next block (or the last chunk's stores,
+      // which are younger still and make the wait stronger): at most 8 outstanding means that block i has landed
+      if (i + 1 < n) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (any) shared_block_compute<TILES>(lds + (b & 1) * SPL_STAGE, (chunk + 8 * c) * ATT_CHUNK + b * ATT_BLOCK, p.qk_scale, qf, qpos, qpos_min, m, l, acc);
+      __syncthreads();  // everyone has read the stage
+      if (i + 2 < n) ld.issue(i + 2, b & 1);
+    }
+    // lane (r16 = query row, g) holds dims 16 f + 4 g .. + 3 of fragment f
 #pragma unroll
-      for (int r = 0; r < 4; r++) ACC[i][r] = fold_add(ACC[i][r], A, acc[0][i][r], B);
-    M = Mn;
+    for (int t = 0; t < TILES; t++) {
+      const int lr = row0 + 16 * (wave * TILES + t);
+      if (lr + r16 >= rows) continue;
+      float* image = sp.shared_part + (((int64_t)(sg.tile0 + (lr >> 4)) * p.Hkv + kvh) * sp.max_chunks + chunk + 8 * c) * sp.shared_floats;
+#pragma unroll
+      for (int f = 0; f < 8; f++)
+        ((float4*)image)[(4 * f + g) * 16 + r16] = make_float4(acc[t][f][0], acc[t][f][1], acc[t][f][2], acc[t][f][3]);
+      if (g == 0) ((float2*)(image + D * 16))[r16] = make_float2(m[t], l[t]);
+    }
   }
-  const int lr = row0 + 16 * wave;
-  if (lr + r16 >= rows) return;
-  float* image = sp.shared_part + ((int64_t)(sg.tile0 + (lr >> 4)) * p.Hkv + kvh) * sp.shared_floats;
-#pragma unroll
-  for (int f = 0; f < 8; f++) ((float4*)image)[(4 * f + g) * 16 + r16] = make_float4(ACC[f][0], ACC[f][1], ACC[f][2], ACC[f][3]);
-  if (g == 0) ((float2*)(image + D * 16))[r16] = make_float2(M, L);
 }
 
 // Launch 2: one workgroup per (sequence, kv head), a thread per (head, 4 dims): shared chunks, then own ones, in ascending
@@ -484,8 +434,7 @@ __global__ __launch_bounds__(256) void attn_shared_fold_kernel(AttnParams p, Sha
   const int d4n = (p.dv + 3) >> 2, nelem = G * d4n;
   const SharedGroup sg = shared_group_of(p, sp, seq);
   const int nch = kv_len > 0 ? (kv_len + ATT_CHUNK - 1) / ATT_CHUNK : 0;
-  const int first = min(sg.chunks, nch);  // a sequence shorter than its group's prefix ends inside it
-  const int ns = sp.walked ? min(first, 1) : first;
+  const int ns = min(sg.chunks, nch);  // a sequence shorter than its group's prefix ends inside it
   for (int e = threadIdx.x; e < nelem; e += blockDim.x) {
     const int hl = e % G, d4 = e / G;
     float4 A4 = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -519,12 +468,12 @@ __global__ __launch_bounds__(256) void attn_shared_fold_kernel(AttnParams p, Sha
     };
     if (ns > 0) {
       const int row = (seq - sg.seq0) * G + hl;
-      const float* image = sp.shared_part + ((int64_t)(sg.tile0 + (row >> 4)) * p.Hkv + kvh) * (sp.walked ? 1 : sp.max_chunks) * sp.shared_floats;
+      const float* image = sp.shared_part + ((int64_t)(sg.tile0 + (row >> 4)) * p.Hkv + kvh) * sp.max_chunks * sp.shared_floats;
       fold(image + ((int64_t)d4 * 16 + (row & 15)) * 4, image + (int64_t)4 * d4n * 16 + 2 * (row & 15), ns, sp.shared_floats);
     }
-    if (nch > first) {
+    if (nch > ns) {
       const float* image = sp.own_part + ((int64_t)seq * p.Hkv + kvh) * sp.max_own * sp.own_floats;
-      fold(image + ((int64_t)d4 * G + hl) * 4, image + (int64_t)4 * d4n * G + 2 * hl, nch - first, sp.own_floats);
+      fold(image + ((int64_t)d4 * G + hl) * 4, image + (int64_t)4 * d4n * G + 2 * hl, nch - ns, sp.own_floats);
     }
     uint2 pk = make_uint2(0u, 0u);
     if (nch > 0) {
@@ -543,31 +492,22 @@ static int launch_shared_prefix_t(const AttnParams& p, SharedParams sp, hipStrea
   constexpr int WAVES = LDS ? 4 : 1;
   // row tiles per wavefront: one where an average group has at most 64 rows, else two
   const int tiles = LDS && rows > 64 * (int64_t)sp.num_groups ? 2 : 1;
-  // Walk the prefixes where that occupies half of the CUs: 64 rows of one kv head per workgroup
-  const bool walk = LDS && rows * p.Hkv >= 64 * 128;
-  sp.walked = walk;
-  sp.blocks = (int)(rows / (16 * WAVES * (walk ? 1 : tiles)) + sp.num_groups);
-  const int64_t swgs = sp.num_groups == 0 || sp.max_chunks == 0 ? 0 : walk ? walk_wgs(sp.blocks, p.Hkv) : shared_wgs(sp.blocks, p.Hkv, sp.max_chunks);
+  sp.blocks = (int)(rows / (16 * WAVES * tiles) + sp.num_groups);
+  // Chunks per workgroup of the LDS form: its set-up (group, block table, queries) costs as much as two chunks, so several
+  // where that leaves about 1536 workgroups (64 sequences on 32768 keys: 138 us with one chunk each, 94 with two, 103 with
+  // four; 16 groups of 16: 153 / 143 / 143)
+  const int64_t units = (int64_t)sp.blocks * p.Hkv * sp.max_chunks;
+  sp.cpw = LDS ? (int)std::max<int64_t>(1, std::min<int64_t>(16, units / 1536)) : 1;
+  const int64_t swgs = sp.num_groups == 0 || sp.max_chunks == 0 ? 0 : shared_wgs(sp.blocks, p.Hkv, sp.max_chunks, sp.cpw);
   // about 4096 wavefronts for the own chunks, at most one per chunk
   sp.splits = (int)std::max<int64_t>(1, std::min<int64_t>((sp.max_own + WAVES - 1) / WAVES, 4096 / (pairs * WAVES)));
   const int64_t owgs = (pairs + 7) / 8 * 8 * sp.splits;
   if (swgs + owgs > 0x7fffffff) return VX_ERR_UNSUPPORTED;
   sp.shared_wgs = (int)swgs;
+  sp.own_wgs = (int)owgs;
   const unsigned grid = (unsigned)(swgs + owgs);
   if constexpr (LDS) {
-    if (walk) {
-      constexpr int LDSB = SPW_STAGES * SPL_STAGE;
-      static DeviceOnce once;
-      const int dev = once.slot();
-      if (once.need(dev)) {
-        if (hipFuncSetAttribute((const void*)attn_shared_walk_kernel<QT, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, LDSB) != hipSuccess) {
-          (void)hipGetLastError();
-          return VX_ERR_LAUNCH;
-        }
-        once.mark(dev);
-      }
-      attn_shared_walk_kernel<QT, KIND><<<grid, 256, LDSB, stream>>>(p, sp);
-    } else if (tiles == 2) attn_shared_chunks_lds_kernel<2, QT, KIND><<<grid, 256, 0, stream>>>(p, sp);
+    if (tiles == 2) attn_shared_chunks_lds_kernel<2, QT, KIND><<<grid, 256, 0, stream>>>(p, sp);
     else attn_shared_chunks_lds_kernel<1, QT, KIND><<<grid, 256, 0, stream>>>(p, sp);
   } else {
     attn_shared_chunks_kernel<ET, DK, DV, QT, KIND, PAD><<<grid, 64, 0, stream>>>(p, sp);

@@ -15,6 +15,7 @@ namespace vx {
 constexpr int VL_BM = 64, VL_BN = 256, VL_BK = 64;
 constexpr int VL_RB = VL_BK * 2 + 16;  // LDS row pitch: 16 bytes on, so that the rows of a fragment read hit distinct banks
 constexpr int VL_SEG = 8192;           // columns per partial sum of d h
+constexpr int VL_FEW = 64;             // rows up to which the forward streams the weights (gemm_stream_kernel)
 
 // The general kernel: any H that is a multiple of 8, any number of rows. 64 rows x 256 columns per workgroup, one
 // 64-column strip per wavefront, operands through registers into one of two LDS buffers.
@@ -97,24 +98,38 @@ __global__ __launch_bounds__(256) void vocab_gemm_kernel(GemmParams p) {
   }
 }
 
-// out = x[label] - lse, lse = M + log S over a row's tile statistics: 8 rows and 32 runs of tiles (s, s + 32, ...) per
-// workgroup, the runs then folded in ascending order.
-__global__ __launch_bounds__(256) void vocab_final_kernel(const float2* __restrict__ part, int64_t part_ld, int ntiles,
-                                                          const float* __restrict__ label_logit, const int64_t* __restrict__ labels,
-                                                          float* __restrict__ out, float* __restrict__ lse_out, int64_t T, int64_t V) {
-  __shared__ float2 red[32][8];
-  const int r = threadIdx.x & 7, s = threadIdx.x >> 3;
-  const int64_t row = (int64_t)blockIdx.x * 8 + r;
+// out = x[label] - lse, lse = M + log S over a row's tile statistics. One wavefront per row, lane r folds the tiles r, r + 64,
+// ... in ascending order, then the lanes fold pairwise (r with r ^ 32, then 16, ... 1). STRIPS: the four strips of a tile
+// come one by one. 16 rows per workgroup: with [tile][row] partials one of its loads then uses whole 128-byte lines.
+template <bool STRIPS>
+__global__ __launch_bounds__(1024) void vocab_final_kernel(const float2* __restrict__ part, int64_t part_ld, int ntiles, int nstrips,
+                                                           const float* __restrict__ label_logit, const int64_t* __restrict__ labels,
+                                                           float* __restrict__ out, float* __restrict__ lse_out, int64_t T, int64_t V) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 6);
+  if (row >= T) return;
   float m = -INFINITY, sum = 0.f;
-  if (row < T)
-    for (int t = s; t < ntiles; t += 32) {
-      const float2 v = part[(int64_t)t * part_ld + row];
-      vocab_fold(m, sum, v.x, v.y);
+#pragma unroll 4
+  for (int t = lane; t < ntiles; t += 64) {
+    float2 a;
+    if constexpr (STRIPS) {
+      float2 st[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) st[j] = 4 * t + j < nstrips ? part[(int64_t)(4 * t + j) * part_ld + row] : make_float2(-INFINITY, 0.f);
+      a = st[0];
+#pragma unroll
+      for (int j = 1; j < 4; j++) vocab_fold(a.x, a.y, st[j].x, st[j].y);
+    } else {
+      a = part[(int64_t)t * part_ld + row];
     }
-  red[s][r] = make_float2(m, sum);
-  __syncthreads();
-  if (s != 0 || row >= T) return;
-  for (int i = 1; i < 32; i++) vocab_fold(m, sum, red[i][r].x, red[i][r].y);
+    vocab_fold(m, sum, a.x, a.y);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(sum, o, 64);
+    vocab_fold(m, sum, m2, s2);
+  }
+  if (lane != 0) return;
   const float ls = logf(sum);
   if (lse_out) lse_out[row] = m + ls;
   if (out) {
@@ -156,6 +171,13 @@ static int launch_vocab_gemm(const GemmParams& p_in, int64_t T, hipStream_t stre
     if (EPI == EPI_LSE) { p.lse_part += r0; p.label_logit += r0; }
     else { p.lse += r0; p.d_out += r0; p.c += r0 * p.ldc; }
     const int64_t tm = ((int64_t)p.M + WD_BM - 1) / WD_BM;
+    if (EPI == EPI_LSE && T <= VL_FEW) {
+      const unsigned nt = (unsigned)(((int64_t)p.N + 63) / 64);
+      if (p.M <= 16) gemm_stream_kernel<1, EPI_LSE, false, 8, 2><<<nt, 256, 0, stream>>>(p);
+      else if (p.M <= 32) gemm_stream_kernel<2, EPI_LSE, false, 8, 2><<<nt, 256, 0, stream>>>(p);
+      else gemm_stream_kernel<4, EPI_LSE, false><<<nt, 256, 0, stream>>>(p);
+      continue;
+    }
     if (p.M > 64 && gemm_wide_launch_t<EPI, false>(p, tm, p.M, stream)) continue;
     const dim3 grid((unsigned)(((int64_t)p.N + VL_BN - 1) / VL_BN), (unsigned)(((int64_t)p.M + VL_BM - 1) / VL_BM));
     vocab_gemm_kernel<EPI><<<grid, 256, 0, stream>>>(p);
@@ -205,7 +227,8 @@ extern "C" {
 
 int64_t vx_vocab_logprobs_workspace_bytes(int64_t T, int64_t V) {
   if (T <= 0 || V <= 0) return 0;
-  return up256((V + 255) / 256 * T * 8) + up256(T * 4);
+  // per 256 columns, or per 64 for a few rows
+  return up256((T <= VL_FEW ? (V + 255) / 256 * 4 : (V + 255) / 256) * T * 8) + up256(T * 4);
 }
 
 int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* labels, float* out, float* lse, int64_t T, int64_t V,
@@ -220,7 +243,8 @@ int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* lab
   p.ldw = ldw; p.K = (int)H;
   p.labels = labels; p.scale = scale; p.tokens = V;
   p.lse_part = (float2*)workspace; p.part_ld = T;
-  p.label_logit = (float*)((uint8_t*)workspace + up256(ntiles * T * 8));
+  const bool few = T <= VL_FEW;
+  p.label_logit = (float*)((uint8_t*)workspace + up256((few ? 4 * ntiles : ntiles) * T * 8));
   for (int64_t v0 = 0; v0 < V; v0 += step) {
     p.w = (const bf16_t*)weight + v0 * ldw;
     p.N = (int)std::min(step, V - v0);
@@ -228,7 +252,10 @@ int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* lab
     const int rc = launch_vocab_gemm<EPI_LSE>(p, T, stream);
     if (rc != VX_OK) return rc;
   }
-  vocab_final_kernel<<<(unsigned)((T + 7) / 8), 256, 0, stream>>>(p.lse_part, T, (int)ntiles, p.label_logit, labels, out, lse, T, V);
+  const unsigned grid = (unsigned)((T + 15) / 16);
+  const int nstrips = (int)((V + 63) / 64);
+  if (few) vocab_final_kernel<true><<<grid, 1024, 0, stream>>>(p.lse_part, T, (int)ntiles, nstrips, p.label_logit, labels, out, lse, T, V);
+  else vocab_final_kernel<false><<<grid, 1024, 0, stream>>>(p.lse_part, T, (int)ntiles, nstrips, p.label_logit, labels, out, lse, T, V);
   return launch_status();
 }
 
