@@ -40,9 +40,9 @@ struct GemmParams {
   const int* row_scale_idx;     //   row_scale[row_scale_idx[i]] (idx null = identity)
   // EPI_LSE / EPI_DLOGITS (vocab_logprob.h): logits are scale * acc; column n of this launch is token vocab_base + n
   const int64_t* labels;  // [M]
-  float2* lse_part;       // EPI_LSE: (max, sum) of 256 columns, [ceil(V / 256)][part_ld]
+  float2* lse_part;       // EPI_LSE: (max, sum) of 256 columns (a few rows: 64), [ceil(V / 256)][part_ld]
   int64_t part_ld;
-  float* label_logit;     // EPI_LSE: [M], the logit of the row's label
+  float* label_logit;     // EPI_LSE: [M], the logit of the row's label, in units of log 2
   const float* lse;       // EPI_DLOGITS: [M]
   const float* d_out;     // EPI_DLOGITS: [M]
   float scale;
@@ -50,7 +50,7 @@ struct GemmParams {
   int64_t tokens;         // the whole vocabulary
 };
 
-__device__ __forceinline__ void vocab_strip(const GemmParams& p, float (&v)[16], int row, bool live, int col0, float2* dst);  // vocab_logprob.h
+__device__ __forceinline__ void vocab_strip(const GemmParams& p, float (&v)[16], int row, int64_t label, int col0, float2* dst);  // vocab_logprob.h
 
 __device__ __forceinline__ float silu_f32(float g) { return g / (1.0f + expf(-g)); }
 
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * NW) void gemm_stream_kernel(GemmParams p) {
         for (int c = 0; c < 4; c++) v[4 * e + c] = q[c];
       }
       float2 st;
-      vocab_strip(p, v, row0 + m, m < rows, blockIdx.x * 64, &st);
+      vocab_strip(p, v, row0 + m, m < rows ? p.labels[row0 + m] : -1, blockIdx.x * 64, &st);
       if (g == 0 && m < rows) p.lse_part[(int64_t)((p.vocab_base >> 6) + blockIdx.x) * p.part_ld + row0 + m] = st;
     }
     return;

@@ -300,6 +300,14 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
       }
     } else if constexpr (EPI == EPI_LSE || EPI == EPI_DLOGITS) {
       float2* strips = (float2*)(wd_lds + 2 * STAGE);  // EPI_LSE: [4][BM] behind the stages
+      int64_t label[EPI == EPI_LSE ? XI : 1];
+      VocabRow vrow[EPI == EPI_DLOGITS ? XI : 1];
+#pragma unroll
+      for (int i = 0; i < XI; i++) {
+        const int m = 16 * XI * wm + 16 * i + r16;
+        if constexpr (EPI == EPI_LSE) label[i] = m < t.rows ? p.labels[t.row0 + m] : -1;
+        else vrow[i] = vocab_row(p, t.row0 + m, m < t.rows);
+      }
 #pragma unroll
       for (int i = 0; i < XI; i++) {
         const int m = 16 * XI * wm + 16 * i + r16;
@@ -309,8 +317,8 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
           v[e] = acc[i][e >> 2][e & 3];
           acc[i][e >> 2][e & 3] = 0.f;
         }
-        if constexpr (EPI == EPI_LSE) vocab_strip(p, v, t.row0 + m, m < t.rows, t.n0 + 64 * wn, strips + wn * BM + m);
-        else vocab_dlogits(p, v, t.row0 + m, m < t.rows, t.n0 + 64 * wn);
+        if constexpr (EPI == EPI_LSE) vocab_strip(p, v, t.row0 + m, label[i], t.n0 + 64 * wn, strips + wn * BM + m);
+        else vocab_dlogits(p, v, t.row0 + m, m < t.rows, vrow[i], t.n0 + 64 * wn);
       }
       if constexpr (EPI == EPI_LSE) {
         // the barriers of the next tile's steps keep its strips from overwriting what is read here

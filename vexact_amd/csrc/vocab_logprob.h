@@ -18,40 +18,45 @@ namespace vx {
 
 constexpr float VL_LOG2E = 1.44269504f;
 
-// Columns col0 + 16 g .. + 15 (g = lane / 16) of row `row` (this launch's numbering) in v: the strip's statistics go to
-// *dst, the label's logit to its place. All 64 lanes call it; `live`: the row exists.
-__device__ __forceinline__ void vocab_strip(const GemmParams& p, float (&v)[16], int row, bool live, int col0, float2* dst) {
+// Columns col0 + 16 g .. + 15 (g = lane / 16) of row `row` (this launch's numbering) in v, unscaled; label: the row's label
+// (anything below 0 for a row that does not exist). The strip's statistics go to *dst, in units of log 2: the maximum m
+// of c v with c = scale log2 e, and the sum of 2^(c v - m), each term one fused multiply-add (m is rounded: 2^-24 |m| in
+// lse) and one exponential; the label's logit goes to its place. All 64 lanes call it.
+__device__ __forceinline__ void vocab_strip(const GemmParams& p, float (&v)[16], int row, int64_t label, int col0, float2* dst) {
   const int g = (threadIdx.x & 63) >> 4;
   const int c0 = col0 + 16 * g;
-  int hit = -1;  // the label's place among the 16
-  if (live) {
-    const int64_t lab = p.labels[row] - p.vocab_base;
-    if (lab >= c0 && lab < c0 + 16 && lab < p.N) hit = (int)(lab - c0);
-  }
-  float m = -INFINITY;
+  const float c = p.scale * VL_LOG2E;
+  const int64_t at = label - p.vocab_base - c0;  // the label's place among the 16
+  if (__ballot(label >= 0 && at >= 0 && at < 16 && c0 + at < p.N)) {  // one strip in some thousand per row
 #pragma unroll
-  for (int e = 0; e < 16; e++) {
-    v[e] *= p.scale;
-    if (e == hit) p.label_logit[row] = v[e];
-    if (c0 + e >= p.N) v[e] = -INFINITY;
-    m = fmaxf(m, v[e]);
+    for (int e = 0; e < 16; e++)
+      if (label >= 0 && e == at && c0 + e < p.N) p.label_logit[row] = v[e] * c;
   }
+  if (col0 + 64 > p.N) {  // wave-uniform: the vocabulary ends inside the strip
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+      if (c0 + e >= p.N) v[e] = -INFINITY;
+  }
+  float m = v[0];
+#pragma unroll
+  for (int e = 1; e < 16; e++) m = fmaxf(m, v[e]);
   m = fmaxf(m, __shfl_xor(m, 16, 64));
   m = fmaxf(m, __shfl_xor(m, 32, 64));
+  m *= c;
   const float ms = m == -INFINITY ? 0.f : m;  // no column, or nothing but -inf (0) and NaN (NaN)
   float s = 0.f;
 #pragma unroll
-  for (int e = 0; e < 16; e++) s += __builtin_amdgcn_exp2f((v[e] - ms) * VL_LOG2E);
+  for (int e = 0; e < 16; e++) s += __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], c, -ms));
   s += __shfl_xor(s, 16, 64);
   s += __shfl_xor(s, 32, 64);
   if (g == 0) *dst = make_float2(m, s);
 }
 
-// (m, s) += (m2, s2), both relative to their own maximum
+// (m, s) += (m2, s2), both relative to their own maximum (in units of log 2)
 __device__ __forceinline__ void vocab_fold(float& m, float& s, float m2, float s2) {
   const float mn = fmaxf(m, m2);
   const float ms = mn == -INFINITY ? 0.f : mn;
-  s = s * __builtin_amdgcn_exp2f((m - ms) * VL_LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - ms) * VL_LOG2E);
+  s = s * __builtin_amdgcn_exp2f(m - ms) + s2 * __builtin_amdgcn_exp2f(m2 - ms);
   m = mn;
 }
 
@@ -63,33 +68,49 @@ __device__ __forceinline__ void vocab_fold_strips(const GemmParams& p, const flo
   p.lse_part[(int64_t)((p.vocab_base + n0) >> 8) * p.part_ld + row] = a;
 }
 
-// The same 16 columns: their derivatives, zeros past the last column, to C (rows of p.ldc, whole 256-column tiles).
-__device__ __forceinline__ void vocab_dlogits(const GemmParams& p, const float (&v)[16], int row, bool live, int col0) {
-  if (!live) return;
+// What a row's derivatives need: its factor -d_out scale and lse / log 2; a label outside the vocabulary has no gradient,
+// whatever d_out holds.
+struct VocabRow {
+  int64_t label;  // in this launch's columns
+  float d, lse2;
+  bool has;
+};
+__device__ __forceinline__ VocabRow vocab_row(const GemmParams& p, int row, bool live) {
+  VocabRow r = {-1, 0.f, 0.f, false};
+  if (live) {
+    const int64_t label = p.labels[row];
+    r.has = label >= 0 && label < p.tokens;
+    r.label = label - p.vocab_base;
+    r.d = r.has ? p.d_out[row] * p.scale : 0.f;
+    r.lse2 = r.has ? p.lse[row] * VL_LOG2E : 0.f;
+  }
+  return r;
+}
+// The same 16 columns: their derivatives, zeros past the last column, to C (rows of p.ldc, whole 64-column strips).
+__device__ __forceinline__ void vocab_dlogits(const GemmParams& p, const float (&v)[16], int row, bool live, const VocabRow& r, int col0) {
   const int g = (threadIdx.x & 63) >> 4;
   const int c0 = col0 + 16 * g;
-  if (c0 >= p.ldc) return;
-  const int64_t label = p.labels[row];
-  const int64_t lab = label - p.vocab_base;
-  // a label outside the vocabulary has no gradient, whatever d_out holds
-  const bool has = label >= 0 && label < p.tokens;
-  const float d = has ? p.d_out[row] * p.scale : 0.f;
-  const float lse = has ? p.lse[row] : 0.f;
-  uint32_t w[8];
+  const float c = p.scale * VL_LOG2E;
+  const int64_t at = r.label - c0;
+  float o[16];
 #pragma unroll
-  for (int h = 0; h < 8; h++) {
-    float o[2];
+  for (int e = 0; e < 16; e++) o[e] = -r.d * __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], c, -r.lse2));
+  if (__ballot(r.has && at >= 0 && at < 16)) {
 #pragma unroll
-    for (int c = 0; c < 2; c++) {
-      const int e = 2 * h + c;
-      const float prob = __builtin_amdgcn_exp2f((v[e] * p.scale - lse) * VL_LOG2E);
-      o[c] = has && c0 + e < p.N ? d * ((lab == c0 + e ? 1.f : 0.f) - prob) : 0.f;
-    }
-    w[h] = pack_bf16x2(o[0], o[1]);
+    for (int e = 0; e < 16; e++)
+      if (r.has && e == at) o[e] = r.d * (1.f - __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], c, -r.lse2)));
   }
+  if (col0 + 64 > p.N || __ballot(!r.has)) {  // the vocabulary ends inside the strip, or a row without a gradient (its
+#pragma unroll                                // logits may be NaN or infinite)
+    for (int e = 0; e < 16; e++)
+      if (!r.has || c0 + e >= p.N) o[e] = 0.f;
+  }
+  if (!live || c0 >= p.ldc) return;
   uint4* cp = (uint4*)(p.c + (int64_t)row * p.ldc + c0);
-  cp[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  cp[1] = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+    cp[h] = make_uint4(pack_bf16x2(o[8 * h], o[8 * h + 1]), pack_bf16x2(o[8 * h + 2], o[8 * h + 3]),
+                       pack_bf16x2(o[8 * h + 4], o[8 * h + 5]), pack_bf16x2(o[8 * h + 6], o[8 * h + 7]));
 }
 
 }  // namespace vx

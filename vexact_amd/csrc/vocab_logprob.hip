@@ -89,8 +89,8 @@ __global__ __launch_bounds__(256) void vocab_gemm_kernel(GemmParams p) {
     float v[16];
 #pragma unroll
     for (int e = 0; e < 16; e++) v[e] = acc[i][e >> 2][e & 3];
-    if constexpr (EPI == EPI_LSE) vocab_strip(p, v, row0 + m, m < rows, n0 + 64 * wave, &strips[wave][m]);
-    else vocab_dlogits(p, v, row0 + m, m < rows, n0 + 64 * wave);
+    if constexpr (EPI == EPI_LSE) vocab_strip(p, v, row0 + m, m < rows ? p.labels[row0 + m] : -1, n0 + 64 * wave, &strips[wave][m]);
+    else vocab_dlogits(p, v, row0 + m, m < rows, vocab_row(p, row0 + m, m < rows), n0 + 64 * wave);
   }
   if constexpr (EPI == EPI_LSE) {
     __syncthreads();
@@ -130,11 +130,11 @@ __global__ __launch_bounds__(1024) void vocab_final_kernel(const float2* __restr
     vocab_fold(m, sum, m2, s2);
   }
   if (lane != 0) return;
-  const float ls = logf(sum);
-  if (lse_out) lse_out[row] = m + ls;
+  const float ls = __builtin_amdgcn_logf(sum);  // log2, as m
+  if (lse_out) lse_out[row] = (m + ls) * 0.693147181f;
   if (out) {
     const int64_t lab = labels[row];
-    out[row] = lab >= 0 && lab < V ? (label_logit[row] - m) - ls : NAN;
+    out[row] = lab >= 0 && lab < V ? ((label_logit[row] - m) - ls) * 0.693147181f : NAN;
   }
 }
 
