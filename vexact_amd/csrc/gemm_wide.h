@@ -83,6 +83,9 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
   constexpr int XBYTES = BM * WD_BK * 2;
   constexpr int STAGE = XBYTES + WD_BN * WD_BK * 2;
   static_assert(XI == 8 || XI == 4, "wavefront tile heights");
+  constexpr bool VOCAB = EPI == EPI_LSE || EPI == EPI_DLOGITS;
+  constexpr int ROWINFO = 4 * BM * 4;  // VOCAB: per-row values of a tile, two of them behind the stages
+  [[maybe_unused]] int row_par = 0;
 
   const int N = p.N, K = p.K;
   const int tiles = tiles_m * tiles_n;
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
   };
   int ld_lin = first, ld_k = 0;
   set_load_tile(tile_at(first));
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t)wd_lds + wave * 1024;
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(lptr_t)wd_lds, lds0 = lds_base + wave * 1024;
   // EPI_SWIGLU: weight rows 8 q .. 8 q + 7 of load instruction q = wave + 8 j have bit 3 of the row
   // index equal to the parity of the wavefront, which says gate or up
   const bf16_t* wsrc = (EPI == EPI_SWIGLU && !PACKED && (wave & 1)) ? p.w2 : p.w;
@@ -251,6 +254,22 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
   for (int lin = first; lin < tiles; lin += G) {
     const WideTile t = tile_at(lin);
     if (!t.ok) break;
+    if constexpr (VOCAB) {
+      // what the epilogue needs of the tile's rows, dword by dword to LDS, so that it waits for no memory: labels (lower,
+      // upper half), d_out, lse. The first step's wait and barrier cover these loads; the other half of the buffer may
+      // still be read by wavefronts that are behind.
+      const uint32_t dst = lds_base + 2 * STAGE + row_par * ROWINFO;
+      const int part = wave % (BM / 64), which = wave / (BM / 64);  // 64 rows; labels or (EPI_DLOGITS) the two floats
+      const int r = t.row0 + min(64 * part + lane, t.rows - 1);
+      if (which == 0) {
+        const uint32_t* lp = (const uint32_t*)(p.labels + r);
+        lds_load4_v(dst + 256 * part, lp);
+        lds_load4_v(dst + 4 * BM + 256 * part, lp + 1);
+      } else if (EPI == EPI_DLOGITS && which == 1) {
+        lds_load4_v(dst + 8 * BM + 256 * part, p.d_out + r);
+        lds_load4_v(dst + 12 * BM + 256 * part, p.lse + r);
+      }
+    }
     for (int kt = 0; kt < nk; kt++) {
       const uint8_t* cur_sb = wd_lds + st * STAGE;
       const uint8_t* oth_sb = wd_lds + (st ^ 1) * STAGE;
@@ -299,27 +318,27 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
         }
       }
     } else if constexpr (EPI == EPI_LSE || EPI == EPI_DLOGITS) {
-      float2* strips = (float2*)(wd_lds + 2 * STAGE);  // EPI_LSE: [4][BM] behind the stages
-      int64_t label[EPI == EPI_LSE ? XI : 1];
-      VocabRow vrow[EPI == EPI_DLOGITS ? XI : 1];
+      float2* strips = (float2*)(wd_lds + 2 * STAGE + 2 * ROWINFO);  // EPI_LSE: [4][BM]
+      const uint32_t* info = (const uint32_t*)(wd_lds + 2 * STAGE + row_par * ROWINFO);
 #pragma unroll
       for (int i = 0; i < XI; i++) {
         const int m = 16 * XI * wm + 16 * i + r16;
-        if constexpr (EPI == EPI_LSE) label[i] = m < t.rows ? p.labels[t.row0 + m] : -1;
-        else vrow[i] = vocab_row(p, t.row0 + m, m < t.rows);
-      }
-#pragma unroll
-      for (int i = 0; i < XI; i++) {
-        const int m = 16 * XI * wm + 16 * i + r16;
+        const bool live = m < t.rows;
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; e++) {
           v[e] = acc[i][e >> 2][e & 3];
           acc[i][e >> 2][e & 3] = 0.f;
         }
-        if constexpr (EPI == EPI_LSE) vocab_strip(p, v, t.row0 + m, label[i], t.n0 + 64 * wn, strips + wn * BM + m);
-        else vocab_dlogits(p, v, t.row0 + m, m < t.rows, vrow[i], t.n0 + 64 * wn);
+        const int64_t label = live ? (int64_t)((uint64_t)info[m] | ((uint64_t)info[BM + m] << 32)) : -1;
+        if constexpr (EPI == EPI_LSE) {
+          vocab_strip(p, v, t.row0 + m, label, t.n0 + 64 * wn, strips + wn * BM + m);
+        } else {
+          const VocabRow r = vocab_row(p, label, __builtin_bit_cast(float, info[2 * BM + m]), __builtin_bit_cast(float, info[3 * BM + m]));
+          vocab_dlogits(p, v, t.row0 + m, live, r, t.n0 + 64 * wn);
+        }
       }
+      row_par ^= 1;
       if constexpr (EPI == EPI_LSE) {
         // the barriers of the next tile's steps keep its strips from overwriting what is read here
         __syncthreads();
@@ -374,8 +393,9 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
 template <int EPI, bool GROUPED, int XI = 8, bool PACKED = false>
 static inline bool gemm_wide_launch_t(const GemmParams& p, int64_t tiles_m, int64_t x_rows, hipStream_t stream) {
   constexpr int NOUT = (EPI == EPI_SWIGLU) ? 128 : 256;
-  // two stages of an activation and a weight tile, and the row statistics of four 64-column strips
-  constexpr int LDS = 2 * (32 * XI + WD_BN) * WD_BK * 2 + (EPI == EPI_LSE ? 4 * 32 * XI * 8 : 0);
+  // two stages of an activation and a weight tile; per-row values of two tiles, row statistics of four 64-column strips
+  constexpr int LDS = 2 * (32 * XI + WD_BN) * WD_BK * 2 + (EPI == EPI_LSE || EPI == EPI_DLOGITS ? 2 * 4 * 32 * XI * 4 : 0) +
+                      (EPI == EPI_LSE ? 4 * 32 * XI * 8 : 0);
   if (p.K % WD_BK != 0 || p.N <= 0 || tiles_m <= 0 || x_rows <= 0) return false;
   const int64_t lim = (int64_t)1 << 32;
   // bytes of one group's weights that a load offset must reach (PACKED: 16-row blocks of p.ldw 1 KB chunks)

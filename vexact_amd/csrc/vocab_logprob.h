@@ -75,15 +75,12 @@ struct VocabRow {
   float d, lse2;
   bool has;
 };
-__device__ __forceinline__ VocabRow vocab_row(const GemmParams& p, int row, bool live) {
-  VocabRow r = {-1, 0.f, 0.f, false};
-  if (live) {
-    const int64_t label = p.labels[row];
-    r.has = label >= 0 && label < p.tokens;
-    r.label = label - p.vocab_base;
-    r.d = r.has ? p.d_out[row] * p.scale : 0.f;
-    r.lse2 = r.has ? p.lse[row] * VL_LOG2E : 0.f;
-  }
+__device__ __forceinline__ VocabRow vocab_row(const GemmParams& p, int64_t label, float d_out, float lse) {
+  VocabRow r;
+  r.has = label >= 0 && label < p.tokens;
+  r.label = label - p.vocab_base;
+  r.d = r.has ? d_out * p.scale : 0.f;
+  r.lse2 = r.has ? lse * VL_LOG2E : 0.f;
   return r;
 }
 // The same 16 columns: their derivatives, zeros past the last column, to C (rows of p.ldc, whole 64-column strips).

@@ -89,8 +89,14 @@ __global__ __launch_bounds__(256) void vocab_gemm_kernel(GemmParams p) {
     float v[16];
 #pragma unroll
     for (int e = 0; e < 16; e++) v[e] = acc[i][e >> 2][e & 3];
-    if constexpr (EPI == EPI_LSE) vocab_strip(p, v, row0 + m, m < rows ? p.labels[row0 + m] : -1, n0 + 64 * wave, &strips[wave][m]);
-    else vocab_dlogits(p, v, row0 + m, m < rows, vocab_row(p, row0 + m, m < rows), n0 + 64 * wave);
+    const bool live = m < rows;
+    const int64_t label = live ? p.labels[row0 + m] : -1;
+    if constexpr (EPI == EPI_LSE) {
+      vocab_strip(p, v, row0 + m, label, n0 + 64 * wave, &strips[wave][m]);
+    } else {
+      const VocabRow r = vocab_row(p, label, live ? p.d_out[row0 + m] : 0.f, live ? p.lse[row0 + m] : 0.f);
+      vocab_dlogits(p, v, row0 + m, live, r, n0 + 64 * wave);
+    }
   }
   if constexpr (EPI == EPI_LSE) {
     __syncthreads();
