@@ -108,7 +108,7 @@ int vx_logprobs_static(const void* logits, const int64_t* labels, float* out, in
  * (standalone_logprobs.py:28-55).
  * The backward recomputes x in pieces of the vocabulary: d_hidden [T, H] and / or d_weight [V, H] (bf16, row strides
  * multiples of 4, either may be null), from the forward's lse and d_out [T] fp32. Rows whose label is outside the
- * vocabulary have no gradient, whatever their d_out. The derivative of each logit is rounded to bf16 once before the
+ * vocabulary have no gradient and leave none in d_weight, whatever they and their d_out hold. The derivative of each logit is rounded to bf16 once before the
  * two products, which accumulate in fp32; no atomics, results repeat bit for bit. T <= 2^32 / 16384 rows. */
 int64_t vx_vocab_logprobs_workspace_bytes(int64_t T, int64_t V);
 int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* labels, float* out, float* lse, int64_t T,

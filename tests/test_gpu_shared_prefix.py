@@ -122,6 +122,21 @@ def test_long_tails_and_many_groups():
 
 
 @gpu
+def test_pages_beyond_four_gib():
+    """Cache offsets past 32 bits: only the last pages of a 4.6 GB cache are in use."""
+    a = make([3, 2], [700, 300], [5, 270], (8, 2), (128, 128), 16, seed=11)
+    n = a["k_cache"].shape[0]
+    blocks = (1 << 32) // (16 * 2 * 128 * 2) + 2 * n
+    for name in ("k_cache", "v_cache"):
+        big = torch.empty(blocks, 16, 2, 128, dtype=torch.bfloat16, device="cuda")
+        big[-n:] = a[name]
+        a[name] = big
+    used = a["page_table"] < (1 << 30)
+    a["page_table"][used] += blocks - n
+    assert_bitwise(ops.shared_prefix_attention(**a), paged(a, decode_kernel="split"))
+
+
+@gpu
 def test_a_full_decode_batch():
     a = make([16] * 16, [1024 + 96 * i for i in range(16)], list(range(1, 600, 37)), (32, 4), (128, 128), 16, seed=3, head_major=True)
     assert_bitwise(ops.shared_prefix_attention(**a), paged(a))

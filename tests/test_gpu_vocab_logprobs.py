@@ -151,6 +151,47 @@ def test_strided_operands_and_special_rows():
     assert torch.isnan(ops.vocab_logprobs(h.cuda(), w.cuda(), none)[0]).all()
     dh, dw = ops.vocab_logprobs_backward(h.cuda(), w.cuda(), none, lse, torch.full((T,), float("nan")).cuda())
     assert not dh.any() and not dw.any()
+    # padding rows may hold anything: nothing of it reaches d_weight or the other rows
+    y2, h3 = y.clone(), h.clone()
+    y2[[2, 5, 69]] = torch.tensor([-100, -1, V])
+    h3[2], h3[5], h3[69] = float("nan"), float("inf"), float("-inf")
+    clean = h.clone()
+    clean[[2, 5, 69]] = 0
+    got, want = [], []
+    for hh, dst in ((h3, got), (clean, want)):
+        _, ls = ops.vocab_logprobs(hh.cuda(), w.cuda(), y2.cuda())
+        dst.extend(ops.vocab_logprobs_backward(hh.cuda(), w.cuda(), y2.cuda(), ls, torch.ones(T).cuda()))
+    assert torch.isfinite(got[1]).all() and not got[0][[2, 5, 69]].any()
+    for a, b in zip(got, want):
+        assert_bitwise(a, b, "padding rows")
+
+
+@gpu
+def test_weights_beyond_four_gib():
+    """Byte offsets past 32 bits, in the forward's column ranges and the backward's pieces."""
+    T, V, H = 70, 270000, 8192
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.randn(V, H, generator=g, device="cuda", dtype=torch.bfloat16) * 0.02
+    h = torch.randn(T, H, generator=g, device="cuda", dtype=torch.bfloat16)
+    y = torch.randint(0, V, (T,), generator=g, device="cuda")
+    y[:3] = torch.tensor([V - 1, 0, V - 300])
+    x = torch.cat([h.float() @ part.float().t() for part in w.split(30000)], 1)
+    lse_ref = torch.logsumexp(x.double(), 1)
+    lp_ref = x.gather(1, y[:, None])[:, 0].double() - lse_ref
+    # fp32 sums of 8192 products on both sides: sqrt(8192) 2^-24 of the root sum of squares of the products (about 1.8) is
+    # 1e-5; ten times that for the largest of the rows
+    for rows in (5, T):
+        out, lse = ops.vocab_logprobs(h[:rows], w, y[:rows])
+        assert (out.double() - lp_ref[:rows]).abs().max() <= 1e-4 and (lse.double() - lse_ref[:rows]).abs().max() <= 1e-4
+    d = torch.randn(T, generator=g, device="cuda")
+    dh, dw = ops.vocab_logprobs_backward(h, w, y, lse, d)
+    dx = -torch.exp(x - lse_ref[:, None].float()) * d[:, None]
+    dx.scatter_add_(1, y[:, None], d[:, None])
+    dh_ref = sum(dx[:, i : i + 30000] @ w[i : i + 30000].float() for i in range(0, V, 30000))
+    assert (dh.float() - dh_ref).norm() <= 2.0**-7 * dh_ref.norm()
+    for i in (0, V - 300, V - 1):
+        ref = dx[:, i] @ h.float()
+        assert (dw[i].float() - ref).norm() <= 2.0**-7 * ref.norm()
 
 
 @gpu

@@ -5,6 +5,8 @@
 //   backward: per piece of the vocabulary, GEMM with the derivative as its epilogue into a bf16 piece [T, piece], then
 //             d W rows of the piece = piece^T h, and fp32 partial sums of d h per segment of 8192 columns, folded in
 //             ascending order. The segments are at absolute positions, so the bits do not depend on the piece width.
+#include <algorithm>
+
 #include "gemm_core.h"
 #include "gemm_seg.h"
 #include "gemm_wide.h"
@@ -162,6 +164,19 @@ __global__ __launch_bounds__(256) void vocab_dh_kernel(const float* __restrict__
   }
 }
 
+// The rows that d W multiplies the derivatives with: those without a label as zeros. Their derivatives are zeros, and a
+// padded row may hold anything, NaN times 0 among it. Eight elements per thread.
+__global__ __launch_bounds__(256) void vocab_rows_kernel(const bf16_t* __restrict__ h, int64_t ldh, const int64_t* __restrict__ labels,
+                                                         bf16_t* __restrict__ out, int64_t T, int H, int64_t V) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = H / 8;
+  const int64_t row = i / per;
+  if (row >= T) return;
+  const int col = (int)(i - row * per) * 8;
+  const int64_t label = labels[row];
+  *(uint4*)(out + row * H + col) = ldg16(h + row * ldh + col, label >= 0 && label < V);
+}
+
 // Logit products of the columns [0, N) of this launch's weights for all rows; row chunks keep the wide kernel's 32-bit
 // offsets in range.
 template <int EPI>
@@ -205,23 +220,27 @@ static int64_t vocab_cols_limit(int64_t V, int64_t H, int64_t ldw) {
 static inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // The backward's piece: segments per piece so that the piece and its partial sums stay near 768 MB (the whole
-// vocabulary at once up to some hundred rows, one segment at a time from some ten thousand).
+// vocabulary at once up to some hundred rows, one segment at a time from some ten thousand) and the piece's weights
+// within the kernels' 32-bit offsets.
 struct VocabPlan {
   int64_t segs, per, pieces, ld;  // segments of the vocabulary, of a piece; pieces; columns of the piece buffer
-  int64_t dlog_bytes, part_bytes, acc_bytes;
+  int64_t dlog_bytes, part_bytes, acc_bytes, rows_bytes;
+  int64_t bytes() const { return dlog_bytes + part_bytes + acc_bytes + rows_bytes; }
 };
-static VocabPlan vocab_plan(int64_t T, int64_t V, int64_t H) {
+static VocabPlan vocab_plan(int64_t T, int64_t V, int64_t H, int64_t ldw) {
   VocabPlan q;
   q.segs = (V + VL_SEG - 1) / VL_SEG;
   const int64_t seg_bytes = T * VL_SEG * 2 + T * H * 4;
-  const int64_t most = std::max<int64_t>(1, std::min(q.segs, ((int64_t)768 << 20) / std::max<int64_t>(1, seg_bytes)));
+  const int64_t reach = ((((int64_t)1 << 32) - 1) / 2 - H) / (VL_SEG * ldw);
+  const int64_t most = std::max<int64_t>(1, std::min({q.segs, ((int64_t)768 << 20) / seg_bytes, reach}));
   q.pieces = (q.segs + most - 1) / most;
   q.per = (q.segs + q.pieces - 1) / q.pieces;
   q.pieces = (q.segs + q.per - 1) / q.per;
   q.ld = std::min(q.per * VL_SEG, (V + 63) / 64 * 64);
   q.dlog_bytes = up256(T * q.ld * 2);
   q.part_bytes = up256(q.per * T * H * 4);
-  q.acc_bytes = q.pieces > 1 ? up256(T * H * 4) : 0;
+  q.acc_bytes = up256(T * H * 4);
+  q.rows_bytes = up256(T * H * 2);
   return q;
 }
 
@@ -267,8 +286,7 @@ int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* lab
 
 int64_t vx_vocab_logprobs_bwd_workspace_bytes(int64_t T, int64_t V, int64_t H) {
   if (T <= 0 || V <= 0 || H <= 0) return 0;
-  const VocabPlan q = vocab_plan(T, V, H);
-  return q.dlog_bytes + q.part_bytes + q.acc_bytes;
+  return vocab_plan(T, V, H, H).bytes();  // a larger row pitch only makes for more, smaller pieces
 }
 
 int vx_vocab_logprobs_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* lse, const float* d_out,
@@ -277,13 +295,16 @@ int vx_vocab_logprobs_bwd(const void* hidden, const void* weight, const int64_t*
   if (!hidden || !weight || !labels || !lse || !d_out || (!d_hidden && !d_weight) || T <= 0 || V <= 0 || H <= 0) return VX_ERR_ARG;
   if (!vocab_args_ok(hidden, weight, T, V, H, ldh, ldw)) return VX_ERR_UNSUPPORTED;
   if ((d_hidden && (ld_dh % 4 || ((uintptr_t)d_hidden & 7))) || (d_weight && (ld_dw % 4 || ((uintptr_t)d_weight & 7)))) return VX_ERR_UNSUPPORTED;
-  const VocabPlan q = vocab_plan(T, V, H);
+  const VocabPlan q = vocab_plan(T, V, H, ldw);
   const int64_t lim = (int64_t)1 << 32;
   if ((T * q.ld + VL_SEG) * 2 >= lim || (q.per * VL_SEG * ldw + H) * 2 >= lim || (T * H / 4 + 255) / 256 > 0x7fffffff) return VX_ERR_UNSUPPORTED;
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < q.dlog_bytes + q.part_bytes + q.acc_bytes) return VX_ERR_WORKSPACE;
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < q.bytes()) return VX_ERR_WORKSPACE;
   bf16_t* dlog = (bf16_t*)workspace;
   float* part = (float*)((uint8_t*)workspace + q.dlog_bytes);
-  float* acc = (float*)((uint8_t*)workspace + q.dlog_bytes + q.part_bytes);
+  float* acc = (float*)((uint8_t*)part + q.part_bytes);
+  bf16_t* rows = (bf16_t*)((uint8_t*)acc + q.acc_bytes);
+  if (d_weight)
+    vocab_rows_kernel<<<(unsigned)((T * (H / 8) + 255) / 256), 256, 0, stream>>>((const bf16_t*)hidden, ldh, labels, rows, T, (int)H, V);
   for (int64_t i = 0; i < q.pieces; i++) {
     const int64_t v0 = i * q.per * VL_SEG, cols = std::min(q.per * VL_SEG, V - v0);
     const bf16_t* w = (const bf16_t*)weight + v0 * ldw;
@@ -302,7 +323,7 @@ int vx_vocab_logprobs_bwd(const void* hidden, const void* weight, const int64_t*
           part, (int)((cols + VL_SEG - 1) / VL_SEG), T * H, acc, i == 0, last ? (bf16_t*)d_hidden : nullptr, ld_dh, T, (int)H);
     }
     if (d_weight) {
-      rc = launch_gemm_tn_rows(dlog, q.ld, (const bf16_t*)hidden, ldh, (bf16_t*)d_weight + v0 * ld_dw, ld_dw, T,
+      rc = launch_gemm_tn_rows(dlog, q.ld, rows, H, (bf16_t*)d_weight + v0 * ld_dw, ld_dw, T,
                                (cols + 63) / 64 * 64, cols, H, stream);
       if (rc != VX_OK) return rc;
     }

@@ -325,13 +325,13 @@ def vocab_logprobs_backward(hidden: torch.Tensor, weight: torch.Tensor, labels: 
                             d_out: torch.Tensor, temperature: float = 1.0, *, need_hidden: bool = True, need_weight: bool = True):
     """``(d_hidden, d_weight)`` (bf16, None where not needed) of ``vocab_logprobs(hidden, weight, labels, temperature)[0]``
     given its ``lse`` and the incoming ``d_out [T]``. The logits are computed again in pieces of the vocabulary; rows
-    without a valid label have no gradient."""
+    without a valid label have no gradient and leave none in ``d_weight``, whatever they hold."""
     x, w, lab, scale = _vocab_operands(hidden, weight, labels, temperature)
     (T, H), V = x.shape, w.shape[0]
     d_x = _empty((T, H), dtype=x.dtype, device=x.device) if need_hidden else None
     d_w = _empty((V, H), dtype=w.dtype, device=w.device) if need_weight else None
-    if lse.dtype != torch.float32 or lse.numel() != T or d_out.numel() != T:
-        raise ValueError("vocab_logprobs: lse (fp32, the forward's) and d_out must have one entry per row")
+    if lse.dtype != torch.float32 or lse.numel() != T or d_out.numel() != T or lse.device != x.device or d_out.device != x.device:
+        raise ValueError("vocab_logprobs: lse (fp32, the forward's) and d_out must have one entry per row, on the rows' device")
     if T == 0 or not (need_hidden or need_weight):
         return d_x, d_w.zero_() if need_weight else None
     ls, g = lse.reshape(-1).contiguous(), d_out.reshape(-1).float().contiguous()
