@@ -208,6 +208,34 @@ def test_other_stream_and_replayed_capture():
         assert_bitwise(out, eager, f"replay {step}")
 
 
+@gpu
+def test_attention_wrapper_with_prefix_groups():
+    """Through the interface a model calls: a step with prefix groups in the context gives the bits of one without."""
+    from types import SimpleNamespace
+
+    from vexact_amd.batch_invariant_ops import flash_attention_forward
+    from vexact_amd.batch_invariant_ops.kv_cache_context import PrefixGroups, clear_kv_cache_context, set_kv_cache_context
+
+    a = make([5, 2], [600, 300], [40, 7, 300], (8, 2), (128, 128), 16, seed=12)
+    B = a["q"].shape[0]
+    a["page_table"][a["page_table"] == 1 << 30] = -1  # padded as the step metadata pads it
+    q = a["q"].transpose(0, 1).unsqueeze(0)  # [1, heads, tokens, dim]
+    new = torch.randn(1, 2, B, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    last = (a["seqused_k"] - 1).long()
+    slots = (a["page_table"].gather(1, (last // 16)[:, None])[:, 0] * 16 + last % 16).int()
+    outs = []
+    for groups in (None, PrefixGroups(a["group_offsets"], a["prefix_lens"], 600)):
+        set_kv_cache_context(is_paged_attn=True, key_cache={0: a["k_cache"]}, value_cache={0: a["v_cache"]}, block_tables=a["page_table"],
+                             context_lens=a["seqused_k"], slot_mapping=slots, query_start_loc=a["cu_seqlens_q"], max_seqlen_q=1, prefix_groups=groups)
+        try:
+            with torch.no_grad():
+                outs.append(flash_attention_forward(SimpleNamespace(layer_idx=0), q, new, new, None, 128**-0.5)[0])
+        finally:
+            clear_kv_cache_context()
+    assert outs[0].shape == (B, 8, 128)
+    assert_bitwise(outs[1], outs[0])
+
+
 def test_refusals():
     z = torch.zeros
     with pytest.raises(ValueError, match="CUDA tensor"):

@@ -224,6 +224,10 @@ def flash_attention_forward(
         if have_kv:  # this step's keys and values go into the cache first
             rows = [t if t.stride(-1) == 1 and t.stride(1) == t.shape[-1] else t.contiguous() for t in (k, v)]
             ops.store_kvcache(rows[0], rows[1], k_blocks, v_blocks, kv_ctx.slot_mapping)
+        groups = kv_ctx.prefix_groups
+        if groups is not None and kv_ctx.max_seqlen_q == 1 and dropout == 0.0 and not torch.is_grad_enabled():
+            return ops.shared_prefix_attention(_addressable(q), k_blocks, v_blocks, kv_ctx.query_start_loc, kv_ctx.context_lens,
+                                               kv_ctx.block_tables, groups.offsets, groups.lens, scaling, max_prefix_len=groups.max_len), None
         return flash_attn_varlen_func(
             q, k_blocks, v_blocks, cu_seqlens_q=kv_ctx.query_start_loc, max_seqlen_q=kv_ctx.max_seqlen_q,
             seqused_k=kv_ctx.context_lens, page_table=kv_ctx.block_tables, dropout_p=dropout, softmax_scale=scaling,

@@ -30,13 +30,25 @@ class KVCacheInfo:
     dtype: torch.dtype = torch.bfloat16
 
 
+@dataclass(frozen=True)
+class PrefixGroups:
+    """Sequences of a decode step that share the pages of a prefix (answers to one prompt): group ``g`` holds the sequences
+    ``offsets[g] .. offsets[g + 1] - 1`` (int32 ``[G + 1]``), whose block tables name the same pages for their first
+    ``lens[g]`` keys (int32 ``[G]``); ``max_len`` bounds ``lens`` from above. No counterpart in the reference."""
+
+    offsets: torch.Tensor
+    lens: torch.Tensor
+    max_len: Optional[int] = None
+
+
 @dataclass
 class KVCacheContext:
     """What the attention wrapper needs for one forward pass.
 
     ``block_tables [B, max_blocks]`` int32 (-1 padded), ``slot_mapping [T]`` int32 (-1 = do not
     store), ``context_lens [B]`` int32 (past + new tokens), ``query_start_loc [B+1]`` int32,
-    ``max_seqlen_q`` host int.
+    ``max_seqlen_q`` host int. ``prefix_groups``: a decode step (``max_seqlen_q == 1``) then reads every shared prefix
+    once per group, with the same bits.
     """
 
     is_paged_attn: bool = False
@@ -47,6 +59,7 @@ class KVCacheContext:
     context_lens: Optional[torch.Tensor] = None
     query_start_loc: Optional[torch.Tensor] = None
     max_seqlen_q: Optional[int] = None
+    prefix_groups: Optional[PrefixGroups] = None
 
     def __post_init__(self):
         if self.is_paged_attn:
@@ -68,6 +81,7 @@ def set_kv_cache_context(
     slot_mapping: Optional[torch.Tensor] = None,
     query_start_loc: Optional[torch.Tensor] = None,
     max_seqlen_q: Optional[int] = None,
+    prefix_groups: Optional[PrefixGroups] = None,
 ):
     _context_storage.kv_cache_context = KVCacheContext(
         is_paged_attn=is_paged_attn,
@@ -78,6 +92,7 @@ def set_kv_cache_context(
         slot_mapping=slot_mapping,
         query_start_loc=query_start_loc,
         max_seqlen_q=max_seqlen_q,
+        prefix_groups=prefix_groups,
     )
 
 
