@@ -309,7 +309,7 @@ __device__ __forceinline__ void shared_load_queries(const AttnParams& p, const S
 
 // One 64-key block from its LDS stage (keys, then values, laid out as attn_prefill_lds_kernel has them): scores, online
 // softmax and P V of TILES 16-row tiles.
-template <int TILES>
+template <class ET, int TILES>
 __device__ __forceinline__ void shared_block_compute(const uint8_t* ks, int kb, float scale, const uint4 (&qf)[TILES][4], const int (&qpos)[TILES],
                                                    const int (&qpos_min)[TILES], float (&m)[TILES], float (&l)[TILES], f32x4 (&acc)[TILES][8]) {
   constexpr int KS = 4;
@@ -326,12 +326,12 @@ __device__ __forceinline__ void shared_block_compute(const uint8_t* ks, int kb, 
     for (int tt = 0; tt < 4; tt++) {
       const uint4 kfr = *(const uint4*)(ks + (16 * tt + r16) * 256 + (((4 * s + g) ^ r16) * 16));
 #pragma unroll
-      for (int t = 0; t < TILES; t++) st[t][tt] = mfma16(kfr, qf[t][s], st[t][tt]);
+      for (int t = 0; t < TILES; t++) st[t][tt] = ET::mfma(kfr, qf[t][s], st[t][tt]);
     }
   uint4 pf[TILES][2];
 #pragma unroll
   for (int t = 0; t < TILES; t++)
-    attn_softmax_tile<ElemBF16>(st[t], kb, scale, qpos[t], m[t], l[t], acc[t], pf[t], kb + ATT_BLOCK - 1 <= qpos_min[t]);
+    attn_softmax_tile<ET>(st[t], kb, scale, qpos[t], m[t], l[t], acc[t], pf[t], kb + ATT_BLOCK - 1 <= qpos_min[t]);
 #pragma unroll
   for (int ch = 0; ch < 2; ch++)
 #pragma unroll
@@ -345,19 +345,19 @@ __device__ __forceinline__ void shared_block_compute(const uint8_t* ks, int kb, 
       const uint2 lo2 = __builtin_bit_cast(uint2, lo), hi2 = __builtin_bit_cast(uint2, hi);
       const uint4 vf = make_uint4(lo2.x, lo2.y, hi2.x, hi2.y);
 #pragma unroll
-      for (int t = 0; t < TILES; t++) acc[t][f] = mfma16(vf, pf[t][ch], acc[t][f]);
+      for (int t = 0; t < TILES; t++) acc[t][f] = ET::mfma(vf, pf[t][ch], acc[t][f]);
     }
 }
 
-// Launch 1 for bf16 heads of 128: the chunk's keys and values are shared by the workgroup through LDS: 4 wavefronts with TILES
+// Launch 1 for heads of 128: the chunk's keys and values are shared by the workgroup through LDS: 4 wavefronts with TILES
 // 16-row tiles each, 64-key blocks brought in by direct-to-LDS loads into one of two 32 KB stages (two workgroups on a
 // CU cover each other's waits), operands, softmax and P V as in attn_prefill_lds_kernel (same layouts and swizzles, same
 // bits). Every wavefront loads the 16 keys of one tile of the block. A chunk is read once per 64 TILES query rows.
-template <int TILES, int QT, int KIND>
+template <class ET, int TILES, int QT, int KIND>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_chunks_lds_kernel(AttnParams p, SharedParams sp) {
   const int index = shared_kind(sp);
   if (index < 0) {
-    attn_own_chunks<ElemBF16, 128, 128, QT, KIND, 4, false>(p, sp, -1 - index);
+    attn_own_chunks<ET, 128, 128, QT, KIND, 4, false>(p, sp, -1 - index);
     return;
   }
   constexpr int D = 128, KS = D / 32, RB = 64 * TILES;
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       if (i + 1 < n) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (any) shared_block_compute<TILES>(lds + (b & 1) * SPL_STAGE, (chunk + 8 * c) * ATT_CHUNK + b * ATT_BLOCK, p.qk_scale, qf, qpos, qpos_min, m, l, acc);
+      if (any) shared_block_compute<ET, TILES>(lds + (b & 1) * SPL_STAGE, (chunk + 8 * c) * ATT_CHUNK + b * ATT_BLOCK, p.qk_scale, qf, qpos, qpos_min, m, l, acc);
       __syncthreads();  // everyone has read the stage
       if (i + 2 < n) ld.issue(i + 2, b & 1);
     }
@@ -488,7 +488,7 @@ template <class ET, int DK, int DV, int QT, int KIND, bool PAD>
 static int launch_shared_prefix_t(const AttnParams& p, SharedParams sp, hipStream_t stream) {
   const int G = p.Hq / p.Hkv;
   const int64_t rows = (int64_t)p.num_seqs * G, pairs = (int64_t)p.num_seqs * p.Hkv;
-  constexpr bool LDS = ET::kDtype == 0 && DK == 128 && DV == 128 && !PAD;
+  constexpr bool LDS = DK == 128 && DV == 128 && !PAD;
   constexpr int WAVES = LDS ? 4 : 1;
   // row tiles per wavefront: one where an average group has at most 64 rows, else two
   const int tiles = LDS && rows > 64 * (int64_t)sp.num_groups ? 2 : 1;
@@ -507,8 +507,8 @@ static int launch_shared_prefix_t(const AttnParams& p, SharedParams sp, hipStrea
   sp.own_wgs = (int)owgs;
   const unsigned grid = (unsigned)(swgs + owgs);
   if constexpr (LDS) {
-    if (tiles == 2) attn_shared_chunks_lds_kernel<2, QT, KIND><<<grid, 256, 0, stream>>>(p, sp);
-    else attn_shared_chunks_lds_kernel<1, QT, KIND><<<grid, 256, 0, stream>>>(p, sp);
+    if (tiles == 2) attn_shared_chunks_lds_kernel<ET, 2, QT, KIND><<<grid, 256, 0, stream>>>(p, sp);
+    else attn_shared_chunks_lds_kernel<ET, 1, QT, KIND><<<grid, 256, 0, stream>>>(p, sp);
   } else {
     attn_shared_chunks_kernel<ET, DK, DV, QT, KIND, PAD><<<grid, 64, 0, stream>>>(p, sp);
   }
