@@ -44,13 +44,29 @@ struct SharedGroup {
   int chunks;   // whole chunks of keys that are computed once for the group
   int src;      // a sequence of the group that holds all of them: its block table is read
 };
-// All 64 lanes call it. The shared keys end where the longest sequence of the group ends, whatever prefix_len says, so
-// that the block table that is read covers them.
-__device__ __forceinline__ SharedGroup shared_group(const AttnParams& p, const SharedParams& s, int g) {
+// The offsets and prefix lengths of 64 groups from `b` on, one per lane, so that whichever is wanted needs no second round
+// trip to memory.
+struct SharedLane {
+  int seq0, n, prefix;
+};
+__device__ __forceinline__ SharedLane shared_lane(const AttnParams& p, const SharedParams& s, int b) {
+  const int g = b + (threadIdx.x & 63);
+  SharedLane l = {p.num_seqs, 0, 0};
+  if (g < s.num_groups) {
+    const int o0 = s.group_off[g], o1 = s.group_off[g + 1];
+    l.prefix = s.prefix_len[g];
+    l.seq0 = min(max(o0, 0), p.num_seqs);
+    l.n = min(max(o1, l.seq0), p.num_seqs) - l.seq0;
+  }
+  return l;
+}
+// The group in lane `from` of l (group g). All 64 lanes call it. The shared keys end where the longest sequence of the
+// group ends, whatever prefix_len says, so that the block table that is read covers them.
+__device__ __forceinline__ SharedGroup shared_group(const AttnParams& p, const SharedParams& s, const SharedLane& l, int from, int g) {
   const int lane = threadIdx.x & 63;
   SharedGroup r;
-  r.seq0 = min(max(s.group_off[g], 0), p.num_seqs);
-  r.n = min(max(s.group_off[g + 1], r.seq0), p.num_seqs) - r.seq0;
+  r.seq0 = __builtin_amdgcn_readlane(l.seq0, from);
+  r.n = __builtin_amdgcn_readlane(l.n, from);
   r.tile0 = (int)((int64_t)r.seq0 * (p.Hq / p.Hkv) / 16) + g;
   int longest = 0;
   r.src = r.seq0;
@@ -65,33 +81,37 @@ __device__ __forceinline__ SharedGroup shared_group(const AttnParams& p, const S
     }
   }
   // a group of one shares nothing: its keys are read once either way
-  r.chunks = r.n < 2 ? 0 : min(min(max(s.prefix_len[g], 0), longest) / ATT_CHUNK, s.max_chunks);
+  r.chunks = r.n < 2 ? 0 : min(min(max(__builtin_amdgcn_readlane(l.prefix, from), 0), longest) / ATT_CHUNK, s.max_chunks);
   return r;
 }
 // The group of a sequence, with no chunks if it is in none: the last group that starts at or before it. All 64 lanes.
 __device__ __forceinline__ SharedGroup shared_group_of(const AttnParams& p, const SharedParams& s, int seq) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int b = 0; b < s.num_groups; b += 64) n += __popcll(__ballot(b + lane < s.num_groups && s.group_off[min(b + lane, s.num_groups - 1)] <= seq));
+  SharedLane l, hit = {};
+  int from = -1, g = 0;
+  for (int b = 0; b < s.num_groups; b += 64) {
+    l = shared_lane(p, s, b);
+    const int left = s.num_groups - b;
+    const uint64_t at = __ballot(l.seq0 <= seq) & (left < 64 ? (1ull << left) - 1 : ~0ull);
+    if (!at) break;
+    hit = l;
+    from = 63 - __builtin_clzll(at);
+    g = b + from;
+  }
   SharedGroup r = {};
-  if (n > 0) r = shared_group(p, s, n - 1);
+  if (from >= 0) r = shared_group(p, s, hit, from, g);
   if (seq >= r.seq0 + r.n) r.chunks = 0;
   return r;
 }
-// Which group row block `item` (rb rows) belongs to, and its place there; -1 behind the last one. The blocks that the
+// Which group row block `item` (rb rows) belongs to, and its place there; false behind the last one. The blocks that the
 // groups really have are numbered first: the launch has room for a partly filled block per group, and with the unused
 // ones in between (every other one where each group fills exactly one) the dispatcher's fixed round of the shader
 // engines left half of the CUs without work (16 groups of 16: 138 against 91 us). All 64 lanes call it.
-__device__ __forceinline__ int shared_block(const AttnParams& p, const SharedParams& s, int item, int rb, int& place) {
+__device__ __forceinline__ bool shared_block(const AttnParams& p, const SharedParams& s, int item, int rb, SharedGroup& sg, int& place) {
   const int lane = threadIdx.x & 63, G = p.Hq / p.Hkv;
   int base = 0;  // blocks of the groups before this round's
   for (int b = 0; b < s.num_groups; b += 64) {
-    int n = 0;
-    if (b + lane < s.num_groups) {
-      const int s0 = min(max(s.group_off[b + lane], 0), p.num_seqs);
-      n = min(max(s.group_off[b + lane + 1], s0), p.num_seqs) - s0;
-    }
-    const int mine = n < 2 ? 0 : (int)(((int64_t)n * G + rb - 1) / rb);
+    const SharedLane gl = shared_lane(p, s, b);
+    const int mine = gl.n < 2 ? 0 : (int)(((int64_t)gl.n * G + rb - 1) / rb);
     int end = mine;  // inclusive sum over the lanes
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -101,12 +121,13 @@ __device__ __forceinline__ int shared_block(const AttnParams& p, const SharedPar
     const uint64_t after = __ballot(base + end > item);
     if (after) {
       const int l = __builtin_ctzll(after);
-      place = item - base - __shfl(end - mine, l, 64);
-      return b + l;
+      place = item - base - __builtin_amdgcn_readlane(end - mine, l);
+      sg = shared_group(p, s, gl, l, b + l);
+      return true;
     }
-    base += __shfl(end, 63, 64);
+    base += __builtin_amdgcn_readlane(end, 63);
   }
-  return -1;
+  return false;
 }
 
 // Launch 1 holds shared and own workgroups; returns the index within the kind, -1 - index for an own one. They alternate in
@@ -200,9 +221,8 @@ __global__ __launch_bounds__(64) void attn_shared_chunks_kernel(AttnParams p, Sh
   int block, kvh, chunk, place;
   shared_place(sp, index, p.Hkv, block, kvh, chunk);
   const int G = p.Hq / p.Hkv;
-  const int gi = shared_block(p, sp, block, 16, place);
-  if (gi < 0) return;
-  const SharedGroup sg = shared_group(p, sp, gi);
+  SharedGroup sg;
+  if (!shared_block(p, sp, block, 16, sg, place)) return;
   const int row0 = place * 16;
   if (chunk >= sg.chunks || row0 >= sg.n * G) return;
   const int r16 = threadIdx.x & 15;
@@ -365,9 +385,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   int block, kvh, chunk, place;
   shared_place(sp, index, p.Hkv, block, kvh, chunk);
   const int G = p.Hq / p.Hkv;
-  const int gi = shared_block(p, sp, block, RB, place);
-  if (gi < 0) return;
-  const SharedGroup sg = shared_group(p, sp, gi);
+  SharedGroup sg;
+  if (!shared_block(p, sp, block, RB, sg, place)) return;
   const int rows = sg.n * G, row0 = place * RB;
   if (chunk >= sg.chunks || row0 >= rows) return;  // uniform over the block
   constexpr int nb = ATT_CHUNK / ATT_BLOCK;
