@@ -173,6 +173,26 @@ def test_padded_batches():
 
 
 @gpu
+@pytest.mark.parametrize("heads,dims,page", [((8, 2), (128, 128), 16), ((6, 2), (64, 64), 16), ((4, 4), (80, 80), 24)])
+def test_what_lies_behind_a_short_sequence_inside_the_prefix(heads, dims, page):
+    """Sequences that end inside their group's prefix read nothing of the keys behind their end, which for them may hold
+    anything, though others of the group do: infinite keys, NaN and infinite values."""
+    a = make([3, 2], [960, 960], [120], heads, dims, page, seed=9)
+    lens = [1080, 300, 256, 1080, 1]
+    a["seqused_k"] = torch.tensor(lens, dtype=torch.int32).cuda()
+    table = a["page_table"].cpu()
+    for seq, key, kv, value in ((0, 300, "k_cache", float("inf")), (0, 305, "v_cache", float("nan")), (3, 2, "v_cache", float("inf")),
+                                (3, 200, "v_cache", float("nan"))):
+        a[kv][int(table[seq, key // page]), key % page] = value
+    out, want = ops.shared_prefix_attention(**a), paged(a, decode_kernel="split")
+    for i in (1, 2, 4):
+        assert torch.isfinite(want[i]).all()
+        assert_bitwise(out[i], want[i])
+    for i in (0, 3):
+        assert torch.isnan(out[i]).all() and torch.isnan(want[i]).all()
+
+
+@gpu
 def test_extreme_scores_and_strides():
     a = make([6], [1040], [30, 1], (8, 2), (128, 128), 16, seed=6)
     a["q"] = torch.cat([a["q"], a["q"]], dim=1)[:, :8]  # token stride of 16 heads

@@ -5,7 +5,9 @@
 // folded in ascending order, so the bits are those of the decode kernels on the same block tables. What changes is who
 // computes a chunk state: for the whole chunks of a shared prefix the query rows of a group (its sequences times the
 // query heads of a kv head) fill the matrix core's 16 columns together, and the chunk's keys are read once per row block
-// instead of once per sequence. The chunk at a prefix's end is each sequence's own.
+// instead of once per sequence. The chunk at a prefix's end is each sequence's own, and so is the chunk in which a sequence
+// shorter than its group's prefix ends: every row that a shared chunk is computed for, and later read for, sees all of its
+// keys, so nothing is masked there, and keys behind a sequence's end may hold anything.
 //
 // Launch 1: chunk states ("images") of the shared prefixes and, in the same grid behind them, of the sequences' own
 // chunks, so that tails of any length fill the chip while the last prefix chunks run. Launch 2: folds a sequence's
@@ -188,7 +190,7 @@ __device__ __forceinline__ void attn_own_chunks(const AttnParams& p, const Share
   const int nch = (kv_len + ATT_CHUNK - 1) / ATT_CHUNK;
   const int mine = z * WAVES + wave;  // wave-uniform
   if (mine >= nch) return;            // whatever is shared
-  const int first = shared_group_of(p, sp, seq).chunks;
+  const int first = min(shared_group_of(p, sp, seq).chunks, kv_len / ATT_CHUNK);
   if (first + mine >= nch) return;
   AttnWave<ET, DK, DV, QT, PAD> w;
   w.init_sizes(p);
@@ -233,9 +235,9 @@ __global__ __launch_bounds__(64) void attn_shared_chunks_kernel(AttnParams p, Sh
   const int seq = sg.seq0 + row / G, head = kvh * G + row % G;
   const int q0 = p.cu_q[seq], qlen = p.cu_q[seq + 1] - q0;
   const bool ok = row0 + r16 < sg.n * G && qlen > 0;
-  w.qpos[0] = ok ? min(p.seqused_k[seq], p.max_kv) - 1 : -1;
   w.load_q(0, p.q + (int64_t)(ok ? q0 + qlen - 1 : 0) * p.sqt + (int64_t)head * p.sqh, ok);
   const int keys = sg.chunks * ATT_CHUNK;  // every one of them exists
+  w.qpos[0] = keys - 1;
   const KVSource<KIND> src = make_source<KIND>(p, sg.src, kvh, 0, keys);
   w.run_chunk(src, chunk * ATT_CHUNK, (chunk + 1) * ATT_CHUNK, keys, p.qk_scale);
   if (ok) shared_store(w, 0, sp.shared_part + (((int64_t)(sg.tile0 + place) * p.Hkv + kvh) * sp.max_chunks + chunk) * sp.shared_floats, 16, r16, w.dv);
@@ -302,11 +304,9 @@ struct SharedLoader {
   }
 };
 
-// Query rows lr0 .. lr0 + 16 TILES - 1 of a group and kv head as MFMA operands, with their last visible keys (-1: no such
-// row) and the smallest of them per tile (blocks that end at or before it need no mask).
+// Query rows lr0 .. lr0 + 16 TILES - 1 of a group and kv head as MFMA operands.
 template <int TILES>
-__device__ __forceinline__ void shared_load_queries(const AttnParams& p, const SharedGroup& sg, int kvh, int lr0, int keys,
-                                                    uint4 (&qf)[TILES][4], int (&qpos)[TILES], int (&qpos_min)[TILES]) {
+__device__ __forceinline__ void shared_load_queries(const AttnParams& p, const SharedGroup& sg, int kvh, int lr0, uint4 (&qf)[TILES][4]) {
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const int G = p.Hq / p.Hkv, rows = sg.n * G;
 #pragma unroll
@@ -316,22 +316,17 @@ __device__ __forceinline__ void shared_load_queries(const AttnParams& p, const S
     const int seq = sg.seq0 + row / G, head = kvh * G + row % G;
     const int q0 = p.cu_q[seq], qlen = p.cu_q[seq + 1] - q0;
     const bool ok = lr < rows && qlen > 0;
-    qpos[t] = ok ? min(p.seqused_k[seq], p.max_kv) - 1 : -1;
     const bf16_t* qp = p.q + (int64_t)(ok ? q0 + qlen - 1 : 0) * p.sqt + (int64_t)head * p.sqh + 8 * g;
 #pragma unroll
     for (int s = 0; s < 4; s++) qf[t][s] = ldg16(qp + 32 * s, ok);
-    int v = ok ? qpos[t] : keys;  // rows that do not exist need no mask
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-    qpos_min[t] = __builtin_amdgcn_readfirstlane(v);
   }
 }
 
 // One 64-key block from its LDS stage (keys, then values, laid out as attn_prefill_lds_kernel has them): scores, online
 // softmax and P V of TILES 16-row tiles.
 template <class ET, int TILES>
-__device__ __forceinline__ void shared_block_compute(const uint8_t* ks, int kb, float scale, const uint4 (&qf)[TILES][4], const int (&qpos)[TILES],
-                                                   const int (&qpos_min)[TILES], float (&m)[TILES], float (&l)[TILES], f32x4 (&acc)[TILES][8]) {
+__device__ __forceinline__ void shared_block_compute(const uint8_t* ks, float scale, const uint4 (&qf)[TILES][4], float (&m)[TILES],
+                                                   float (&l)[TILES], f32x4 (&acc)[TILES][8]) {
   constexpr int KS = 4;
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const uint8_t* vs = ks + ATT_BLOCK * 256;
@@ -351,7 +346,7 @@ __device__ __forceinline__ void shared_block_compute(const uint8_t* ks, int kb, 
   uint4 pf[TILES][2];
 #pragma unroll
   for (int t = 0; t < TILES; t++)
-    attn_softmax_tile<ET>(st[t], kb, scale, qpos[t], m[t], l[t], acc[t], pf[t], kb + ATT_BLOCK - 1 <= qpos_min[t]);
+    attn_softmax_tile<ET>(st[t], 0, scale, 0, m[t], l[t], acc[t], pf[t], true);  // every key is visible
 #pragma unroll
   for (int ch = 0; ch < 2; ch++)
 #pragma unroll
@@ -402,8 +397,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 
   // ---- this wavefront's query tiles
   uint4 qf[TILES][KS];
-  int qpos[TILES], qpos_min[TILES];
-  shared_load_queries<TILES>(p, sg, kvh, row0 + 16 * wave * TILES, keys, qf, qpos, qpos_min);
+  shared_load_queries<TILES>(p, sg, kvh, row0 + 16 * wave * TILES, qf);
   const bool any = row0 + 16 * wave * TILES < rows;  // wave-uniform: a wavefront without rows only loads
   for (int c = 0; c < mine; c++) {
     float m[TILES], l[TILES];
@@ -423,7 +417,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
       if (i + 1 < n) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (any) shared_block_compute<ET, TILES>(lds + (b & 1) * SPL_STAGE, (chunk + 8 * c) * ATT_CHUNK + b * ATT_BLOCK, p.qk_scale, qf, qpos, qpos_min, m, l, acc);
+      if (any) shared_block_compute<ET, TILES>(lds + (b & 1) * SPL_STAGE, p.qk_scale, qf, m, l, acc);
       __syncthreads();  // everyone has read the stage
       if (i + 2 < n) ld.issue(i + 2, b & 1);
     }
@@ -453,7 +447,7 @@ __global__ __launch_bounds__(256) void attn_shared_fold_kernel(AttnParams p, Sha
   const int d4n = (p.dv + 3) >> 2, nelem = G * d4n;
   const SharedGroup sg = shared_group_of(p, sp, seq);
   const int nch = kv_len > 0 ? (kv_len + ATT_CHUNK - 1) / ATT_CHUNK : 0;
-  const int ns = min(sg.chunks, nch);  // a sequence shorter than its group's prefix ends inside it
+  const int ns = min(sg.chunks, max(kv_len, 0) / ATT_CHUNK);  // a sequence shorter than its group's prefix: whole chunks
   for (int e = threadIdx.x; e < nelem; e += blockDim.x) {
     const int hl = e % G, d4 = e / G;
     float4 A4 = make_float4(0.f, 0.f, 0.f, 0.f);
