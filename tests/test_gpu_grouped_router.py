@@ -157,6 +157,23 @@ def test_strided_logits_rows_alone_and_a_replayed_capture():
 
 
 @gpu
+@pytest.mark.parametrize("E,n", [(8, 4), (512, 64)])
+def test_group_score_that_is_no_number(E, n):
+    """The best two of group 0 are +inf and -inf: their sum is NaN, which ranks with -inf, so the group goes last."""
+    size = E // n
+    bias = torch.zeros(E)
+    bias[:size] = -torch.inf
+    bias[1] = torch.inf
+    x = torch.randn(5, E, generator=torch.Generator().manual_seed(8))
+    _, idx = ops.router_topk_grouped(x.cuda(), 2, score="sigmoid", bias=bias.cuda(), n_groups=n, topk_groups=2)
+    s = torch.sigmoid(x.double()).view(5, n, size)
+    best = s[:, 1:].sort(dim=-1, descending=True).values[..., :2].sum(-1).sort(dim=-1, descending=True).indices[:, :2] + 1
+    ok = torch.zeros(5, n, dtype=torch.bool).scatter_(1, best, True).repeat_interleave(size, 1)
+    want = torch.where(ok, s.view(5, E), -torch.inf).sort(dim=-1, descending=True, stable=True).indices[:, :2]
+    assert torch.equal(idx.cpu(), want)
+
+
+@gpu
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_gradient_against_differences(score):
     T, E, k, eps = 6, 32, 4, 2.0**-9

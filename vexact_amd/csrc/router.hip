@@ -102,7 +102,8 @@ __global__ __launch_bounds__(256) void router_grouped_kernel(RouterParams p) {
       b = fmax(fmin(a, oa), fmax(b, ob));
       a = fmax(a, oa);
     }
-    const double score = p.group_top == 2 && size > 1 ? a + b : a;
+    double score = p.group_top == 2 && size > 1 ? a + b : a;
+    if (!(score == score)) score = -INFINITY;  // +inf and -inf among the best two
     int before = 0;  // groups that come before this lane's
     for (int h = 0; h < p.n_groups; h++) {
       const uint64_t bits = __builtin_bit_cast(uint64_t, score);
