@@ -390,8 +390,8 @@ int vx_router_topk_bwd(const void* logits, const int64_t* idx, const void* d_wei
  * selected s; all of them 0: weights 0). Ties go to the lower index, NaN ranks with -inf; scores and sums are held in
  * 64 bits, so the selection is that of the exact scores. E <= 512, k <= 64, n_groups <= 64, topk_groups groups must
  * hold at least k experts. vx_router_topk is the router of the reference's own block (softmax, no bias, no groups).
- * The backward gives d_logits [T, E] (the logits' type) from idx (int64, distinct within a row; an index outside
- * [0, E) selects nothing) and d_weights [T, k]. */
+ * The backward gives d_logits [T, E] (the logits' type) from idx (int64; an expert named twice in a row has the sum of
+ * both derivatives, an index outside [0, E) selects nothing) and d_weights [T, k]. */
 int vx_router_grouped(const void* logits, const float* bias, void* weights, void* idx, int64_t T, int E, int k,
                       int64_t ld, int sigmoid, int n_groups, int topk_groups, int group_top, int renorm, float scale,
                       int logits_bf16, int weights_bf16, int idx_i64, hipStream_t stream);

@@ -175,6 +175,26 @@ def test_group_score_that_is_no_number(E, n):
 
 @gpu
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_backward_of_an_expert_selected_twice(score, renorm):
+    """A selection of the caller's own may name an expert more than once: its gradients add up."""
+    T, E, k = 9, 96, 6
+    g = torch.Generator().manual_seed(9)
+    x, d = torch.randn(T, E, generator=g), torch.randn(T, k, generator=g)
+    idx = torch.randint(0, 4, (T, k), generator=g) * 30  # six of four experts
+    got = ops.router_topk_grouped_backward(x.cuda(), idx.cuda(), d.cuda(), score=score, renorm=renorm, scale=1.5).cpu().double()
+    X = x.double().requires_grad_()
+    s = torch.softmax(X, 1) if score == "softmax" else torch.sigmoid(X)
+    sel = s.gather(1, idx)
+    w = 1.5 * sel / sel.sum(1, keepdim=True) if renorm else 1.5 * sel
+    (want,) = torch.autograd.grad(w, X, d.double())
+    # one rounding to fp32, and 2^-40 of the terms that may cancel: at most 2 k scale max |d|, as s <= 1 and 1 / S times
+    # a selected score <= 1
+    assert (got - want).abs().le(2.0**-24 * want.abs() + 2.0**-40 * 2 * k * 1.5 * d.abs().max()).all()
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_gradient_against_differences(score):
     T, E, k, eps = 6, 32, 4, 2.0**-9
     x = (torch.randn(T, E, generator=torch.Generator().manual_seed(3)) * 64).round() / 64

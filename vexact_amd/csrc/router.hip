@@ -172,6 +172,7 @@ __global__ __launch_bounds__(256) void router_grouped_bwd_kernel(const void* __r
                                                                  const void* __restrict__ d_w, void* __restrict__ d_logits, int64_t T,
                                                                  int E, int k, int64_t ld, int64_t ldo, int sigmoid, int renorm, float scale) {
   __shared__ double ss[4][64 * PER], ds[4][64 * PER];
+  __shared__ int owner[4][64 * PER];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int64_t t_ = (int64_t)blockIdx.x * 4 + wv;
   const bool live = t_ < T;
@@ -222,7 +223,19 @@ __global__ __launch_bounds__(256) void router_grouped_bwd_kernel(const void* __r
     d = tot == 0.0 ? 0.0 : (d - dot / tot) / tot;
   }
   const double c = wave_sum_f64(at >= 0 ? d * sel : 0.0);
-  if (at >= 0) ds[wv][at] = d;
+  if (at >= 0) { ds[wv][at] = d; owner[wv][at] = lane; }
+  __syncthreads();
+  // an expert that is named twice (never by the forward) has one owner and lanes that lost: then every lane adds up the
+  // derivatives of its expert in ascending order
+  if (__ballot(at >= 0 && owner[wv][at] != lane)) {
+    double sum = 0.0;
+    for (int j = 0; j < k; j++) {
+      const int other = __shfl(at, j, 64);
+      const double dj = __shfl(d, j, 64);
+      if (other == at) sum += dj;
+    }
+    if (at >= 0) ds[wv][at] = sum;
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < PER; i++) {

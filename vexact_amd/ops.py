@@ -952,7 +952,8 @@ def router_topk_grouped(
 
 def router_topk_grouped_backward(logits: torch.Tensor, selected: torch.Tensor, d_weights: torch.Tensor, *,
                                  score: str = "softmax", renorm: bool = True, scale: float = 1.0) -> torch.Tensor:
-    """Gradient of ``router_topk_grouped(logits, k, ...)[0]`` with respect to ``logits [T, E]``, given the selected experts."""
+    """Gradient of ``router_topk_grouped(logits, k, ...)[0]`` with respect to ``logits [T, E]``, given the selected experts
+    (one named twice has the sum of both gradients; entries outside ``[0, E)`` select nothing)."""
     lg = _grouped_router_logits(logits, selected.shape[-1], score)
     T, E = lg.shape
     k = selected.shape[-1]
