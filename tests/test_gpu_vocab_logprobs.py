@@ -167,6 +167,20 @@ def test_strided_operands_and_special_rows():
 
 
 @gpu
+def test_rows_far_apart():
+    """Rows further apart than the kernels' 32-bit offsets of a piece allow: the values of copies that lie close."""
+    T, V, H, pitch = 5, 70, 64, (1 << 18) + 8
+    h, w, y = (t.cuda() for t in make(T, V, H, seed=21))
+    far = lambda t: torch.zeros(len(t), pitch, dtype=t.dtype, device="cuda")[:, :H].copy_(t)  # noqa: E731
+    hf, wf = far(h), far(w)
+    assert hf.stride(0) == wf.stride(0) == pitch
+    d = torch.linspace(-1, 1, T).cuda()
+    near, apart = ops.vocab_logprobs(h, w, y), ops.vocab_logprobs(hf, wf, y)
+    for a, b in zip(near + ops.vocab_logprobs_backward(h, w, y, near[1], d), apart + ops.vocab_logprobs_backward(hf, wf, y, near[1], d)):
+        assert_bitwise(a, b)
+
+
+@gpu
 def test_weights_beyond_four_gib():
     """Byte offsets past 32 bits, in the forward's column ranges and the backward's pieces."""
     T, V, H = 70, 270000, 8192
@@ -319,3 +333,13 @@ def test_c_abi_refusals():
     assert bwd(T=0) == bwd(g=None) == bwd(l=None) == bwd(dh=None, dw=None) == -1
     assert bwd(H=12) == bwd(ldd=18) == bwd(dh=a + 4) == bwd(T=1 << 28, n=1 << 60) == -2
     assert bwd(ws=None) == bwd(n=16) == -3
+
+
+def test_c_abi_refuses_rows_too_far_apart():
+    """A row pitch that no split of the rows or of the vocabulary brings within 32-bit offsets is refused."""
+    from vexact_amd import _lib
+
+    lib, a = _lib.load(), 4096
+    for H, ldh, ldw in ((16, 1 << 23, 16), (16, 16, 1 << 23), (16, 1 << 40, 16), (16, 16, 1 << 40), (1 << 23, 1 << 23, 1 << 23), (16, -16, 16), (16, 16, -16)):
+        assert lib.vx_vocab_logprobs(a, a, a, a, a, 4, 10, H, ldh, ldw, 1.0, a, 1 << 40, None) == -2
+        assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, 4, 10, H, ldh, ldw, H, H, 1.0, a, 1 << 60, None) == -2

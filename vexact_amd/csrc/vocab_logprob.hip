@@ -206,8 +206,12 @@ static int launch_vocab_gemm(const GemmParams& p_in, int64_t T, hipStream_t stre
   return launch_status();
 }
 
+// The kernels address a launch's rows with 32-bit byte offsets: launches of 256 rows or columns, the fewest that these are
+// split into, must stay within them.
+constexpr int64_t VL_MAX_LD = (int64_t)1 << 22;
 static bool vocab_args_ok(const void* h, const void* w, int64_t T, int64_t V, int64_t H, int64_t ldh, int64_t ldw) {
-  return V <= 0x7fffff00 && H <= 0x7fffff00 && T <= 0x7fffff00 && gemm_fast_ok(h, w, H, ldh, ldw);
+  return V <= 0x7fffff00 && T <= 0x7fffff00 && H <= VL_MAX_LD && ldh >= 0 && ldw >= 0 && ldh <= VL_MAX_LD && ldw <= VL_MAX_LD &&
+         gemm_fast_ok(h, w, H, ldh, ldw);
 }
 
 // columns of one launch: whole 256-column tiles, weight bytes within 32 bits

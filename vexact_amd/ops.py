@@ -294,7 +294,8 @@ def _vocab_operands(hidden, weight, labels, temperature):
         raise ValueError("vocab_logprobs: temperature must be positive")
     if hidden.shape[1] % 8 or weight.shape[0] == 0:
         raise ValueError(f"vocab_logprobs: H must be a multiple of 8 and V positive, got H = {hidden.shape[1]}, V = {weight.shape[0]}")
-    aligned = lambda t: t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0  # noqa: E731
+    # rows further apart than this put a piece of the vocabulary beyond the kernels' 32-bit offsets
+    aligned = lambda t: t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= 1 << 17 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0  # noqa: E731
     x, w = (t if aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (hidden, weight))
     return x, w, labels.reshape(-1).to(torch.int64).contiguous(), 1.0 / float(temperature)
 
