@@ -137,6 +137,20 @@ def test_pages_beyond_four_gib():
 
 
 @gpu
+def test_rows_of_a_page_far_apart():
+    """A cache whose outermost dimension is the place in a page: neighbouring keys lie 290 MB apart, a page spans 4.6 GB."""
+    a = make([5], [1040], [40, 3], (8, 2), (128, 128), 16, seed=10)
+    want = paged(a, decode_kernel="split")
+    n = a["k_cache"].shape[0]
+    for name in ("k_cache", "v_cache"):
+        far = torch.empty(16, 570000, 2, 128, dtype=torch.bfloat16, device="cuda").permute(1, 0, 2, 3)
+        far[:n] = a[name]
+        a[name] = far
+    assert 15 * 2 * a["k_cache"].stride(1) > 1 << 32
+    assert_bitwise(ops.shared_prefix_attention(**a), want)
+
+
+@gpu
 def test_a_full_decode_batch():
     a = make([16] * 16, [1024 + 96 * i for i in range(16)], list(range(1, 600, 37)), (32, 4), (128, 128), 16, seed=3, head_major=True)
     assert_bitwise(ops.shared_prefix_attention(**a), paged(a))

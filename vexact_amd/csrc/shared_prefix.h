@@ -534,7 +534,8 @@ static int launch_shared_prefix_t(const AttnParams& p, SharedParams sp, hipStrea
 
 template <class ET, int DK, int DV, bool PAD>
 static int launch_shared_prefix(const AttnParams& p, const SharedParams& sp, hipStream_t stream) {
-  const bool fast = p.page_shift >= 4;  // page size a power of two >= 16
+  // page size a power of two >= 16, and the 16 keys of a tile within SharedLoader's 32-bit offsets
+  const bool fast = p.page_shift >= 4 && std::max(p.skp, p.svp) < (int64_t)1 << 27;
   if (p.Hq / p.Hkv <= 16)
     return fast ? launch_shared_prefix_t<ET, DK, DV, 1, SRC_FAST, PAD>(p, sp, stream) : launch_shared_prefix_t<ET, DK, DV, 1, SRC_GENERIC, PAD>(p, sp, stream);
   return fast ? launch_shared_prefix_t<ET, DK, DV, 2, SRC_FAST, PAD>(p, sp, stream) : launch_shared_prefix_t<ET, DK, DV, 2, SRC_GENERIC, PAD>(p, sp, stream);
