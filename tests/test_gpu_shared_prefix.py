@@ -151,6 +151,21 @@ def test_rows_of_a_page_far_apart():
 
 
 @gpu
+def test_no_groups_and_a_given_workspace():
+    a = make([2, 1], [300, 0], [40, 3, 700], (8, 2), (128, 128), 16, seed=11)
+    a["group_offsets"], a["prefix_lens"] = a["group_offsets"][:1].contiguous(), a["prefix_lens"][:0]
+    want = paged(a, decode_kernel="split")
+    assert_bitwise(ops.shared_prefix_attention(**a), want)
+    for n in (1 << 22, 16):  # enough, and too small: then it is not used
+        ws = torch.full((n,), float("nan"), device="cuda")
+        assert_bitwise(ops.shared_prefix_attention(**a, workspace=ws), want)
+        assert torch.isnan(ws).all() == (n == 16)
+    for ws in (torch.empty(1 << 22), torch.empty(1 << 22, 2, device="cuda")[:, 0]):
+        with pytest.raises(ValueError, match="workspace must be"):
+            ops.shared_prefix_attention(**a, workspace=ws)
+
+
+@gpu
 def test_a_full_decode_batch():
     a = make([16] * 16, [1024 + 96 * i for i in range(16)], list(range(1, 600, 37)), (32, 4), (128, 128), 16, seed=3, head_major=True)
     assert_bitwise(ops.shared_prefix_attention(**a), paged(a))

@@ -751,6 +751,8 @@ def shared_prefix_attention(
             raise ValueError(f"{name} must be an int32 tensor on {q.device} with contiguous entries, got {t.dtype} on {t.device}")
     if k_cache.device != q.device or v_cache.device != q.device or o.device != q.device:
         raise ValueError("q, the caches and out must be on one device")
+    if workspace is not None and (workspace.device != q.device or not workspace.is_contiguous()):
+        raise ValueError("workspace must be a contiguous tensor on q's device")
     if T == 0 or B == 0:
         return o
     width = page_table.shape[1] * page
