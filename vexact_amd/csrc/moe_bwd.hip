@@ -857,8 +857,11 @@ constexpr int NR_STAGES = 4, NR_STAGE = 2 * 64 * 128;
 __global__ __launch_bounds__(256) void gemm_nn_segments_ring_kernel(MoeNnParams p, int tiles_n) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NR_STAGES * NR_STAGE];
   const int tiles_m = (p.M + 63) >> 6;
-  const int seg = blockIdx.x / (tiles_m * tiles_n), rem = blockIdx.x - seg * tiles_m * tiles_n;
-  const int row0 = rem / tiles_n * 64, n0 = rem % tiles_n * 64;
+  // every XCD takes a run of (segment, column tile, row tile) in that order
+  const int per = gridDim.x >> 3, unit = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  const int seg = unit / (tiles_m * tiles_n), rem = unit - seg * tiles_m * tiles_n;
+  if (seg * p.seg_cols >= p.cols) return;
+  const int row0 = rem % tiles_m * 64, n0 = rem / tiles_m * 64;
   const int valid = min(p.seg_cols, p.cols - seg * p.seg_cols), nk = (valid + 63) >> 6;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -991,7 +994,7 @@ int launch_gemm_nn_segments(const bf16_t* a, int64_t lda, const bf16_t* w, int64
   p.cf = out; p.M = (int)M; p.seg_cols = seg_cols; p.cols = (int)cols;
   if (tiles < 64) {  // too few 256 x 256 tiles for the chip
     const int64_t tn64 = (N + 63) / 64, wgs = (M + 63) / 64 * tn64 * ((cols + seg_cols - 1) / seg_cols);
-    gemm_nn_segments_ring_kernel<<<(unsigned)wgs, 256, 0, stream>>>(p, (int)tn64);
+    gemm_nn_segments_ring_kernel<<<(unsigned)((wgs + 7) / 8 * 8), 256, 0, stream>>>(p, (int)tn64);
     return launch_status();
   }
   constexpr int LDS = 2 * 2 * 256 * 64 * 2;
