@@ -56,7 +56,8 @@ def check_forward(h, w, y, out, lse, temperature=1.0):
 # rows on both sides of the kernels' tile heights; vocabularies that end inside a strip, a tile and a segment; depths
 # that are and are not a multiple of the wide kernel's step
 SHAPES = [(1, 1, 8), (1, 5, 64), (3, 64, 64), (7, 257, 72), (64, 1000, 128), (65, 1000, 128), (100, 1024, 136), (129, 8192, 64),
-          (300, 8193, 192), (257, 20011, 128), (513, 16449, 256), (30, 20011, 520)]
+          (300, 8193, 192), (257, 20011, 128), (513, 16449, 256), (30, 20011, 520),
+          (300, 30001, 64), (700, 16449, 512)]
 
 
 @gpu
@@ -89,7 +90,7 @@ def test_backward(T, V, H):
 
 
 @gpu
-@pytest.mark.parametrize("V,H", [(20011, 128), (1000, 72)])
+@pytest.mark.parametrize("V,H", [(20011, 128), (30001, 128), (1000, 72)])
 def test_rows_do_not_depend_on_the_batch(V, H):
     h, w, y = (t.cuda() for t in make(600, V, H, seed=5))
     out, lse = ops.vocab_logprobs(h, w, y)

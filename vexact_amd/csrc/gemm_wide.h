@@ -62,8 +62,8 @@ struct WideTile {
 // fragments 0, 1 and the matching up columns in fragments 2, 3: LDS row 64 wn + 16 a + 4 j + b is
 // column 32 wn + 8 a + 4 (j & 1) + b of gate (j < 2) or up (j >= 2). A tile then yields 128 output
 // columns and a lane 8 consecutive ones per activation row.
-// XI = 16-row activation tiles per wavefront: 8 (256-row tiles, the normal form) or 4 (128-row tiles: the same
-// weight panel and barriers for half the rows, for a last round of tiles that would leave half the chip idle).
+// XI = 16-row activation tiles per wavefront: 8 (256-row tiles, the normal form), 6 or 4 (192- and 128-row tiles: the
+// same weight panel and barriers for fewer rows, where 256-row tiles would be half empty or leave half the chip idle).
 // PACKED: the weights are in fragment order (pack_weights_kernel; p.ldw = 32-wide k-chunks stored per 16-row
 // block; a step advances two chunks = 1024 elements). There 16-byte piece pc (8 k-elements) of the 16 rows of a
 // block is contiguous, so the weight tile lives in LDS piece-major and in fragment order, [pc][position] with
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
   constexpr int NLQ = NXQ + 4;                            // all load instructions per wavefront and step
   constexpr int XBYTES = BM * WD_BK * 2;
   constexpr int STAGE = XBYTES + WD_BN * WD_BK * 2;
-  static_assert(XI == 8 || XI == 4, "wavefront tile heights");
+  static_assert(XI == 8 || XI == 6 || XI == 4, "wavefront tile heights");
   constexpr bool VOCAB = EPI == EPI_LSE || EPI == EPI_DLOGITS;
   constexpr int ROWINFO = 4 * BM * 4;  // VOCAB: per-row values of a tile, two of them behind the stages
   [[maybe_unused]] int row_par = 0;
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(512) void gemm_wide_kernel(GemmParams p, int tiles_
       if constexpr (decltype(LOADS)::value) {
         if (2 * i < NLQ) {
           issue_one(2 * i, ld_stage);
-          issue_one(2 * i + 1, ld_stage);
+          if (2 * i + 1 < NLQ) issue_one(2 * i + 1, ld_stage);
         }
       }
       if (i < 4) {  // two reads beside each of the first four MFMA groups, one beside the others (XI = 8)

@@ -847,21 +847,25 @@ __global__ __launch_bounds__(256) void router_topk_bwd_kernel(const void* __rest
 
 static inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// The segment form for few tiles: 64 x 64 outputs per workgroup, 4 wavefronts of 32 x 32, both operands directly to LDS into a
-// ring of four 16 KB stages of 64 contraction rows (three steps of loads in flight; two workgroups on a CU). Rows are 128
+// The segment form for few tiles: 32 RT x 64 outputs per workgroup, 4 wavefronts of 16 RT x 32, both operands directly to LDS
+// into a ring of four stages of 64 contraction rows (three steps of loads in flight; two workgroups on a CU). Rows are 128
 // bytes in both tiles; 16-byte piece c of activation row r at c ^ (r / 2) % 8, and of weight row r at c ^ 2 f(r), f = bit 1
 // of r and bit 3 above it: the eight rows that a transposing read touches at a time then start at eight different 32-byte
-// slots. Same MFMA chain per output as the 256 x 256 kernel. 300 rows x 32003 tokens x 1024: 169 -> 54 us, where the wide
-// kernel has 32 tiles for 256 CUs; four times the L2 traffic makes it level near 64 of them.
-constexpr int NR_STAGES = 4, NR_STAGE = 2 * 64 * 128;
+// slots. Same MFMA chain per output as the 256 x 256 kernel. 300 rows x 32003 tokens x 1024: 169 -> 41 us, where the wide
+// kernel has 32 tiles for 256 CUs; four times the L2 traffic makes it level near 64 of them. Bound by what a CU brings
+// into LDS, 29 bytes a clock: a step takes 234 ns at 16 KB, 277 at 20, 350 at 24, with four stages as with eight, with 64
+// workgroups as with 192, and with the operand reads of the next step beside the products.
+constexpr int NR_STAGES = 4;
+template <int RT>
 __global__ __launch_bounds__(256) void gemm_nn_segments_ring_kernel(MoeNnParams p, int tiles_n) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[NR_STAGES * NR_STAGE];
-  const int tiles_m = (p.M + 63) >> 6;
+  constexpr int BM = 32 * RT, XB = BM * 128, STAGE = XB + 64 * 128;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int tiles_m = (p.M + BM - 1) / BM;
   // every XCD takes a run of (segment, column tile, row tile) in that order
   const int per = gridDim.x >> 3, unit = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   const int seg = unit / (tiles_m * tiles_n), rem = unit - seg * tiles_m * tiles_n;
   if (seg * p.seg_cols >= p.cols) return;
-  const int row0 = rem % tiles_m * 64, n0 = rem / tiles_m * 64;
+  const int row0 = rem % tiles_m * BM, n0 = rem / tiles_m * 64;
   const int valid = min(p.seg_cols, p.cols - seg * p.seg_cols), nk = (valid + 63) >> 6;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -869,60 +873,61 @@ __global__ __launch_bounds__(256) void gemm_nn_segments_ring_kernel(MoeNnParams 
   const bf16_t* a = p.a[0] + (int64_t)seg * p.seg_cols;
   const bf16_t* w = p.w[0] + (int64_t)seg * p.w_gstride[0];
   const int64_t ldw = p.ldw[0];
-  // load instruction q = wave + 4 t: rows [8 (q % 8), + 8) of the activation (t < 2) or weight tile
+  // load instruction t: rows [8 (wave + 4 t), + 8) of the activation (t < RT) or weight tile (from t = RT)
   auto wswz = [](int r) { return (((r >> 1) & 1) | ((r >> 2) & 2)) << 1; };
-  uint32_t off[4];
+  uint32_t off[RT + 2];
   int wcol[2];
 #pragma unroll
-  for (int t = 0; t < 4; t++) {
-    const int R = 8 * ((wave + 4 * t) & 7) + (lane >> 3), slot = lane & 7;
-    if (t < 2) {
+  for (int t = 0; t < RT + 2; t++) {
+    const int R = 8 * (wave + 4 * (t < RT ? t : t - RT)) + (lane >> 3), slot = lane & 7;
+    if (t < RT) {
       off[t] = (uint32_t)(((int64_t)min(row0 + R, p.M - 1) * p.lda[0] + 8 * (slot ^ nn_swz_x(R))) * 2);
     } else {
-      wcol[t - 2] = min(n0 + 8 * (slot ^ wswz(R)), p.N - 8);  // columns past N re-read the last piece
-      off[t] = (uint32_t)(((int64_t)R * ldw + wcol[t - 2]) * 2);
+      wcol[t - RT] = min(n0 + 8 * (slot ^ wswz(R)), p.N - 8);  // columns past N re-read the last piece
+      off[t] = (uint32_t)(((int64_t)R * ldw + wcol[t - RT]) * 2);
     }
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t)lds;
   auto issue = [&](int step) {  // past the last step it is read again into a stage that nobody reads
     const int s = min(step, nk - 1);
-    const uint32_t dst = lds0 + (step & (NR_STAGES - 1)) * NR_STAGE;
+    const uint32_t dst = lds0 + (step & (NR_STAGES - 1)) * STAGE;
     const bool ragged = 64 * s + 64 > valid;  // rows past the segment's last one re-read it
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
+    for (int t = 0; t < RT + 2; t++) {
       uint32_t o = off[t];
-      if (t >= 2 && ragged) {
-        const int R = 8 * ((wave + 4 * t) & 7) + (lane >> 3);
-        o = (uint32_t)(((int64_t)min(R, valid - 1 - 64 * s) * ldw + wcol[t - 2]) * 2);
+      if (t >= RT && ragged) {
+        const int R = 8 * (wave + 4 * (t - RT)) + (lane >> 3);
+        o = (uint32_t)(((int64_t)min(R, valid - 1 - 64 * s) * ldw + wcol[t - RT]) * 2);
       }
-      lds_load16_sv(dst + (t < 2 ? 0 : 64 * 128) + ((wave + 4 * t) & 7) * 1024, o, t < 2 ? a + 64 * s : w + (int64_t)64 * s * ldw);
+      lds_load16_sv(dst + (wave + 4 * t) * 1024, o, t < RT ? a + 64 * s : w + (int64_t)64 * s * ldw);
     }
   };
-  f32x4 acc[2][2];  // [activation tile][weight fragment]
+  f32x4 acc[RT][2];  // [activation tile][weight fragment]
 #pragma unroll
-  for (int i = 0; i < 2; i++)
+  for (int i = 0; i < RT; i++)
 #pragma unroll
     for (int j = 0; j < 2; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int xoff = (32 * wm + r16) * 128 + ((g ^ (r16 >> 1)) * 16);
+  const int xoff = (16 * RT * wm + r16) * 128 + ((g ^ (r16 >> 1)) * 16);
   const int wrow = 8 * g + (r16 >> 2);
   int woff[2][2];
 #pragma unroll
   for (int j = 0; j < 2; j++)
 #pragma unroll
     for (int h = 0; h < 2; h++)
-      woff[j][h] = 64 * 128 + (wrow + 4 * h) * 128 + (((4 * wn + 2 * j + ((r16 >> 1) & 1)) ^ wswz(wrow + 4 * h)) << 4) + 8 * (r16 & 1);
+      woff[j][h] = XB + (wrow + 4 * h) * 128 + (((4 * wn + 2 * j + ((r16 >> 1) & 1)) ^ wswz(wrow + 4 * h)) << 4) + 8 * (r16 & 1);
 #pragma unroll
   for (int t = 0; t < NR_STAGES - 1; t++) issue(t);
   for (int s = 0; s < nk; s++) {
-    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // 4 loads per step and wavefront: step s has landed
-    __syncthreads();                                  // for everyone, and everyone is done with step s - 1
+    // RT + 2 loads per step and wavefront, of which those of two steps may be on their way: step s has landed
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NR_STAGES - 2) * (RT + 2)) : "memory");
+    __syncthreads();  // for everyone, and everyone is done with step s - 1
     issue(s + NR_STAGES - 1);
-    const uint8_t* sb = lds + (s & (NR_STAGES - 1)) * NR_STAGE;
-    uint4 xf[2][2], wf[2][2];
+    const uint8_t* sb = lds + (s & (NR_STAGES - 1)) * STAGE;
+    uint4 xf[2][RT], wf[2][2];
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) xf[ks][i] = *(const uint4*)(sb + (xoff ^ (64 * ks)) + i * 2048);
+      for (int i = 0; i < RT; i++) xf[ks][i] = *(const uint4*)(sb + (xoff ^ (64 * ks)) + i * 2048);
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t*)(sb + woff[j][0] + ks * 32 * 128));
@@ -934,15 +939,15 @@ __global__ __launch_bounds__(256) void gemm_nn_segments_ring_kernel(MoeNnParams 
 #pragma unroll
     for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-      for (int i = 0; i < 2; i++)
+      for (int i = 0; i < RT; i++)
 #pragma unroll
         for (int j = 0; j < 2; j++) acc[i][j] = mfma16(wf[ks][j], xf[ks][i], acc[i][j]);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the ring's last loads still target our LDS
-  // lane holds C[row0 + 32 wm + 16 i + r16][n0 + 32 wn + 16 j + 4 g + c]
+  // lane holds C[row0 + 16 RT wm + 16 i + r16][n0 + 32 wn + 16 j + 4 g + c]
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int m = row0 + 32 * wm + 16 * i + r16;
+  for (int i = 0; i < RT; i++) {
+    const int m = row0 + 16 * RT * wm + 16 * i + r16;
     if (m >= p.M) continue;
     float* cp = p.cf + ((int64_t)seg * p.M + m) * p.N;
 #pragma unroll
@@ -979,6 +984,23 @@ static int launch_gemm_tn(MoeTnParams p, int64_t num_experts, int64_t dy_rows, i
   return launch_status();
 }
 
+template <int RT>
+static int launch_nn_segments_ring(const MoeNnParams& p, int64_t M, int64_t tn64, int64_t per_row, hipStream_t stream) {
+  constexpr int LDS = NR_STAGES * (32 * RT + 64) * 128;
+  static DeviceOnce once;
+  const int dev = once.slot();
+  if (LDS > 65536 && once.need(dev)) {
+    if (hipFuncSetAttribute((const void*)gemm_nn_segments_ring_kernel<RT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) {
+      (void)hipGetLastError();
+      return VX_ERR_LAUNCH;
+    }
+    once.mark(dev);
+  }
+  const int64_t wgs = (M + 32 * RT - 1) / (32 * RT) * per_row;
+  gemm_nn_segments_ring_kernel<RT><<<(unsigned)((wgs + 7) / 8 * 8), 256, LDS, stream>>>(p, (int)tn64);
+  return launch_status();
+}
+
 // One dense product over segments of the contraction (gemm_seg.h)
 int launch_gemm_nn_segments(const bf16_t* a, int64_t lda, const bf16_t* w, int64_t ldw, float* out, int64_t M, int64_t N,
                             int64_t cols, int seg_cols, hipStream_t stream) {
@@ -993,9 +1015,12 @@ int launch_gemm_nn_segments(const bf16_t* a, int64_t lda, const bf16_t* w, int64
   p.N = (int)N;
   p.cf = out; p.M = (int)M; p.seg_cols = seg_cols; p.cols = (int)cols;
   if (tiles < 64) {  // too few 256 x 256 tiles for the chip
-    const int64_t tn64 = (N + 63) / 64, wgs = (M + 63) / 64 * tn64 * ((cols + seg_cols - 1) / seg_cols);
-    gemm_nn_segments_ring_kernel<<<(unsigned)((wgs + 7) / 8 * 8), 256, 0, stream>>>(p, (int)tn64);
-    return launch_status();
+    const int64_t tn64 = (N + 63) / 64, per_row = tn64 * ((cols + seg_cols - 1) / seg_cols);
+    // 96 rows where that saves a round of 256 workgroups (300 rows x 32003 x 1024: 44 -> 41 us, 640 rows: 83 -> 63);
+    // otherwise they only make a step longer (100 rows: 30 -> 36 us, 1000 rows x 32003 x 512: 90 -> 106)
+    auto rounds = [&](int64_t bm) { return ((M + bm - 1) / bm * per_row + 255) / 256; };
+    if (rounds(96) < rounds(64)) return launch_nn_segments_ring<3>(p, M, tn64, per_row, stream);
+    return launch_nn_segments_ring<2>(p, M, tn64, per_row, stream);
   }
   constexpr int LDS = 2 * 2 * 256 * 64 * 2;
   static DeviceOnce once;

@@ -177,6 +177,15 @@ __global__ __launch_bounds__(256) void vocab_rows_kernel(const bf16_t* __restric
   *(uint4*)(out + row * H + col) = ldg16(h + row * ldh + col, label >= 0 && label < V);
 }
 
+// Rows of the wide kernel's tiles: those whose rounds of 256 workgroups take least, a tile of 192 or 128 rows counted as
+// 0.85 or 0.7 of one of 256.
+static int vocab_tile_rows(int64_t M, int64_t N) {
+  const int64_t tn = (N + WD_BN - 1) / WD_BN;
+  auto cost = [&](int64_t bm, int64_t weight) { return ((M + bm - 1) / bm * tn + 255) / 256 * weight; };
+  const int64_t c256 = cost(256, 100), c192 = cost(192, 85), c128 = cost(128, 70);
+  return c128 < c192 && c128 < c256 ? 128 : c192 < c256 ? 192 : 256;
+}
+
 // Logit products of the columns [0, N) of this launch's weights for all rows; row chunks keep the wide kernel's 32-bit
 // offsets in range.
 template <int EPI>
@@ -191,7 +200,6 @@ static int launch_vocab_gemm(const GemmParams& p_in, int64_t T, hipStream_t stre
     p.labels += r0;
     if (EPI == EPI_LSE) { p.lse_part += r0; p.label_logit += r0; }
     else { p.lse += r0; p.d_out += r0; p.c += r0 * p.ldc; }
-    const int64_t tm = ((int64_t)p.M + WD_BM - 1) / WD_BM;
     if (EPI == EPI_LSE && T <= VL_FEW) {
       const unsigned nt = (unsigned)(((int64_t)p.N + 63) / 64);
       if (p.M <= 16) gemm_stream_kernel<1, EPI_LSE, false, 8, 2><<<nt, 256, 0, stream>>>(p);
@@ -199,7 +207,15 @@ static int launch_vocab_gemm(const GemmParams& p_in, int64_t T, hipStream_t stre
       else gemm_stream_kernel<4, EPI_LSE, false><<<nt, 256, 0, stream>>>(p);
       continue;
     }
-    if (p.M > 64 && gemm_wide_launch_t<EPI, false>(p, tm, p.M, stream)) continue;
+    if (p.M > 64) {
+      bool done;
+      switch (vocab_tile_rows(p.M, p.N)) {
+        case 128: done = gemm_wide_launch_t<EPI, false, 4>(p, ((int64_t)p.M + 127) / 128, p.M, stream); break;
+        case 192: done = gemm_wide_launch_t<EPI, false, 6>(p, ((int64_t)p.M + 191) / 192, p.M, stream); break;
+        default: done = gemm_wide_launch_t<EPI, false>(p, ((int64_t)p.M + WD_BM - 1) / WD_BM, p.M, stream);
+      }
+      if (done) continue;
+    }
     const dim3 grid((unsigned)(((int64_t)p.N + VL_BN - 1) / VL_BN), (unsigned)(((int64_t)p.M + VL_BM - 1) / VL_BM));
     vocab_gemm_kernel<EPI><<<grid, 256, 0, stream>>>(p);
   }
