@@ -852,7 +852,7 @@ static inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // bytes in both tiles; 16-byte piece c of activation row r at c ^ (r / 2) % 8, and of weight row r at c ^ 2 f(r), f = bit 1
 // of r and bit 3 above it: the eight rows that a transposing read touches at a time then start at eight different 32-byte
 // slots. Same MFMA chain per output as the 256 x 256 kernel. 300 rows x 32003 tokens x 1024: 169 -> 41 us, where the wide
-// kernel has 32 tiles for 256 CUs; four times the L2 traffic makes it level near 64 of them. Bound by what a CU brings
+// kernel has 32 tiles for 256 CUs. Bound by what a CU brings
 // into LDS, 29 bytes a clock: a step takes 234 ns at 16 KB, 277 at 20, 350 at 24, with four stages as with eight, with 64
 // workgroups as with 192, and with the operand reads of the next step beside the products.
 constexpr int NR_STAGES = 4;
@@ -861,11 +861,12 @@ __global__ __launch_bounds__(256) void gemm_nn_segments_ring_kernel(MoeNnParams 
   constexpr int BM = 32 * RT, XB = BM * 128, STAGE = XB + 64 * 128;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int tiles_m = (p.M + BM - 1) / BM;
-  // every XCD takes a run of (segment, column tile, row tile) in that order
+  // every XCD takes a run of (segment, panel of 8 row tiles, column tile, row tile) in that order
   const int per = gridDim.x >> 3, unit = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   const int seg = unit / (tiles_m * tiles_n), rem = unit - seg * tiles_m * tiles_n;
   if (seg * p.seg_cols >= p.cols) return;
-  const int row0 = rem % tiles_m * BM, n0 = rem / tiles_m * 64;
+  const int panel = rem / (8 * tiles_n), in = rem - panel * 8 * tiles_n, high = min(8, tiles_m - 8 * panel);
+  const int row0 = (8 * panel + in % high) * BM, n0 = in / high * 64;
   const int valid = min(p.seg_cols, p.cols - seg * p.seg_cols), nk = (valid + 63) >> 6;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -985,7 +986,7 @@ static int launch_gemm_tn(MoeTnParams p, int64_t num_experts, int64_t dy_rows, i
 }
 
 template <int RT>
-static int launch_nn_segments_ring(const MoeNnParams& p, int64_t M, int64_t tn64, int64_t per_row, hipStream_t stream) {
+static int launch_nn_segments_ring(const MoeNnParams& p, int64_t wgs, int64_t tn64, hipStream_t stream) {
   constexpr int LDS = NR_STAGES * (32 * RT + 64) * 128;
   static DeviceOnce once;
   const int dev = once.slot();
@@ -996,7 +997,6 @@ static int launch_nn_segments_ring(const MoeNnParams& p, int64_t M, int64_t tn64
     }
     once.mark(dev);
   }
-  const int64_t wgs = (M + 32 * RT - 1) / (32 * RT) * per_row;
   gemm_nn_segments_ring_kernel<RT><<<(unsigned)((wgs + 7) / 8 * 8), 256, LDS, stream>>>(p, (int)tn64);
   return launch_status();
 }
@@ -1014,14 +1014,16 @@ int launch_gemm_nn_segments(const bf16_t* a, int64_t lda, const bf16_t* w, int64
   p.a[0] = a; p.lda[0] = lda; p.w[0] = w; p.ldw[0] = ldw; p.w_gstride[0] = seg_cols * ldw;
   p.N = (int)N;
   p.cf = out; p.M = (int)M; p.seg_cols = seg_cols; p.cols = (int)cols;
-  if (tiles < 64) {  // too few 256 x 256 tiles for the chip
-    const int64_t tn64 = (N + 63) / 64, per_row = tn64 * ((cols + seg_cols - 1) / seg_cols);
-    // 96 rows where that saves a round of 256 workgroups (300 rows x 32003 x 1024: 44 -> 41 us, 640 rows: 83 -> 63);
-    // otherwise they only make a step longer (100 rows: 30 -> 36 us, 1000 rows x 32003 x 512: 90 -> 106)
-    auto rounds = [&](int64_t bm) { return ((M + bm - 1) / bm * per_row + 255) / 256; };
-    if (rounds(96) < rounds(64)) return launch_nn_segments_ring<3>(p, M, tn64, per_row, stream);
-    return launch_nn_segments_ring<2>(p, M, tn64, per_row, stream);
-  }
+  // The ring kernel, 96 rows a tile where that saves a round of 256 workgroups (300 rows x 32003 x 1024: 44 -> 41 us, 640
+  // rows: 83 -> 63); otherwise they only make a step longer (100 rows: 30 -> 36 us, 1000 rows x 32003 x 512: 90 -> 106).
+  // A round takes 31 to 36 us with segments of 8192, one of the 256 x 256 kernel 167 whether full or not, so the ring goes
+  // up to 4.5 rounds per round of that (with the logits' derivatives, ring against wide: 1000 rows x 32003 x 1024: 159 /
+  // 227 us, 1500: 228 / 254, 2000: 304 / 281; 64 rows x 151936 x 2048: 286 / 343, 128: 387 / 359).
+  const int64_t tn64 = (N + 63) / 64, per_row = tn64 * ((cols + seg_cols - 1) / seg_cols);
+  const int64_t wgs64 = (M + 63) / 64 * per_row, wgs96 = (M + 95) / 96 * per_row;
+  const bool tall = (wgs96 + 255) / 256 < (wgs64 + 255) / 256;
+  if ((tall ? wgs96 : wgs64) <= 1152 * ((tiles + 255) / 256))
+    return tall ? launch_nn_segments_ring<3>(p, wgs96, tn64, stream) : launch_nn_segments_ring<2>(p, wgs64, tn64, stream);
   constexpr int LDS = 2 * 2 * 256 * 64 * 2;
   static DeviceOnce once;
   const int dev = once.slot();
