@@ -140,3 +140,18 @@ def test_training_on_the_scored_answers():
     # sqrt(12) 2^-8 = 0.014 of a gradient's norm, twice that here
     for n, a, b in zip(("x", *names), got, want):
         assert (a.cpu().double() - b).norm() <= 0.028 * b.norm(), n
+
+
+def test_second_derivatives_are_refused():
+    """The gradients are the kernels' in either mode; a gradient of a gradient says that there is none."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(12, 32, generator=g).cuda().requires_grad_()
+    h = torch.randn(12, 64, generator=g).to(torch.bfloat16).cuda().requires_grad_()
+    w, y = torch.randn(200, 64, generator=g).to(torch.bfloat16).cuda(), torch.randint(0, 200, (12,), generator=g).cuda()
+    for f, leaf in ((lambda: grouped_topk_router(x, 4, out_dtype=torch.float32)[0].square().sum(), x), (lambda: logprobs_from_hidden(h, w, y).square().sum(), h)):
+        (plain,) = torch.autograd.grad(f(), leaf)
+        (again,) = torch.autograd.grad(f(), leaf, create_graph=True)
+        assert_bitwise(again.detach(), plain)
+        assert not plain.requires_grad and again.requires_grad
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            again.float().sum().backward()

@@ -12,6 +12,7 @@ from typing import Optional
 import torch
 
 from .. import ops
+from ._autograd import once_differentiable
 
 
 class _GroupedRouterFunction(torch.autograd.Function):
@@ -30,7 +31,7 @@ class _GroupedRouterFunction(torch.autograd.Function):
         return weights, selected
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, d_weights, _):
         if d_weights is None:
             return (None,) * 10

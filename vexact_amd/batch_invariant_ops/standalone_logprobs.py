@@ -8,6 +8,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
+from ._autograd import once_differentiable
 
 
 class _LogprobsFunction(torch.autograd.Function):
@@ -52,7 +53,7 @@ class _HiddenLogprobsFunction(torch.autograd.Function):
         return out.reshape(labels.shape)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, d_out):
         hidden, weight, labels, lse = ctx.saved_tensors
         need_hidden, need_weight = ctx.needs_input_grad[:2]
