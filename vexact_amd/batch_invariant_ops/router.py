@@ -24,7 +24,7 @@ class _GroupedRouterFunction(torch.autograd.Function):
         weights, selected = ops.router_topk_grouped(
             logits, top_k, score=score, bias=bias, n_groups=n_groups, topk_groups=topk_groups, group_top=group_top,
             renorm=renorm, scale=scale, out_dtype=out_dtype)
-        ctx.save_for_backward(logits, selected)
+        ctx.save_for_backward(logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous(), selected)
         ctx.call = (score, renorm, scale)
         ctx.mark_non_differentiable(selected)
         ctx.set_materialize_grads(False)  # no zeros for the gradient that the selection does not have
@@ -37,8 +37,7 @@ class _GroupedRouterFunction(torch.autograd.Function):
             return (None,) * 10
         logits, selected = ctx.saved_tensors
         score, renorm, scale = ctx.call
-        d_logits = ops.router_topk_grouped_backward(logits, selected, d_weights, score=score, renorm=renorm, scale=scale)
-        return (d_logits, *([None] * 9))
+        return (ops._router_grouped_backward(logits, selected, d_weights, score, renorm, scale), *([None] * 9))
 
 
 def grouped_topk_router(

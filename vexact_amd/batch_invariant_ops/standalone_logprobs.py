@@ -46,20 +46,19 @@ class _HiddenLogprobsFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, labels, temperature):
-        flat = hidden.reshape(-1, hidden.shape[-1])
-        out, lse = ops.vocab_logprobs(flat, weight, labels, temperature)
-        ctx.save_for_backward(hidden, weight, labels, lse)
-        ctx.temperature = temperature
+        x, w, flat_labels, scale = ops._vocab_operands(hidden.reshape(-1, hidden.shape[-1]), weight, labels, temperature)
+        out, lse = ops._vocab_forward(x, w, flat_labels, scale)
+        ctx.save_for_backward(x, w, flat_labels, lse)  # as the kernels take them: nothing to check or copy again
+        ctx.scale, ctx.hidden_shape = scale, hidden.shape
         return out.reshape(labels.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        hidden, weight, labels, lse = ctx.saved_tensors
+        x, w, labels, lse = ctx.saved_tensors
         need_hidden, need_weight = ctx.needs_input_grad[:2]
-        d_hidden, d_weight = ops.vocab_logprobs_backward(hidden.reshape(-1, hidden.shape[-1]), weight, labels, lse, d_out,
-                                                         ctx.temperature, need_hidden=need_hidden, need_weight=need_weight)
-        return d_hidden.reshape(hidden.shape) if need_hidden else None, d_weight, None, None
+        d_hidden, d_weight = ops._vocab_backward(x, w, labels, lse, d_out, ctx.scale, need_hidden, need_weight)
+        return d_hidden.reshape(ctx.hidden_shape) if need_hidden else None, d_weight, None, None
 
 
 def logprobs_from_hidden(

@@ -305,7 +305,10 @@ def vocab_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Ten
     temperature`` (bf16 operands, H a multiple of 8), which never reach memory. A label outside ``[0, V)`` gives NaN. A
     row's bits depend on its own hidden state only; the logits are not rounded to bf16 as those of ``matmul`` are, so
     they are not the bits of ``logprobs(matmul(...))``."""
-    x, w, lab, scale = _vocab_operands(hidden, weight, labels, temperature)
+    return _vocab_forward(*_vocab_operands(hidden, weight, labels, temperature))
+
+
+def _vocab_forward(x, w, lab, scale):
     T, H = x.shape
     out = _empty(T, dtype=torch.float32, device=x.device)
     lse = _empty(T, dtype=torch.float32, device=x.device)
@@ -328,19 +331,24 @@ def vocab_logprobs_backward(hidden: torch.Tensor, weight: torch.Tensor, labels: 
     given its ``lse`` and the incoming ``d_out [T]``. The logits are computed again in pieces of the vocabulary; rows
     without a valid label have no gradient and leave none in ``d_weight``, whatever they hold."""
     x, w, lab, scale = _vocab_operands(hidden, weight, labels, temperature)
+    T = x.shape[0]
+    if lse.dtype != torch.float32 or lse.numel() != T or d_out.numel() != T or lse.device != x.device or d_out.device != x.device:
+        raise ValueError("vocab_logprobs: lse (fp32, the forward's) and d_out must have one entry per row, on the rows' device")
+    return _vocab_backward(x, w, lab, lse.reshape(-1).contiguous(), d_out, scale, need_hidden, need_weight)
+
+
+def _vocab_backward(x, w, lab, lse, d_out, scale, need_hidden, need_weight):
     (T, H), V = x.shape, w.shape[0]
     d_x = _empty((T, H), dtype=x.dtype, device=x.device) if need_hidden else None
     d_w = _empty((V, H), dtype=w.dtype, device=w.device) if need_weight else None
-    if lse.dtype != torch.float32 or lse.numel() != T or d_out.numel() != T or lse.device != x.device or d_out.device != x.device:
-        raise ValueError("vocab_logprobs: lse (fp32, the forward's) and d_out must have one entry per row, on the rows' device")
     if T == 0 or not (need_hidden or need_weight):
         return d_x, d_w.zero_() if need_weight else None
-    ls, g = lse.reshape(-1).contiguous(), d_out.reshape(-1).float().contiguous()
+    g = d_out.reshape(-1).float().contiguous()
     lib = _lib.load()
     with _on_device(x):
         ws = _workspace(lib.vx_vocab_logprobs_bwd_workspace_bytes(T, V, H), x.device)
         _lib.check(
-            lib.vx_vocab_logprobs_bwd(x.data_ptr(), w.data_ptr(), lab.data_ptr(), ls.data_ptr(), g.data_ptr(), _ptr(d_x), _ptr(d_w),
+            lib.vx_vocab_logprobs_bwd(x.data_ptr(), w.data_ptr(), lab.data_ptr(), lse.data_ptr(), g.data_ptr(), _ptr(d_x), _ptr(d_w),
                                       T, V, H, x.stride(0), w.stride(0), H, H, scale, ws.data_ptr(), ws.numel(), _raw_stream(x)),
             "vx_vocab_logprobs_bwd",
         )
@@ -958,12 +966,15 @@ def router_topk_grouped_backward(logits: torch.Tensor, selected: torch.Tensor, d
     """Gradient of ``router_topk_grouped(logits, k, ...)[0]`` with respect to ``logits [T, E]``, given the selected experts
     (one named twice has the sum of both gradients; entries outside ``[0, E)`` select nothing)."""
     lg = _grouped_router_logits(logits, selected.shape[-1], score)
-    T, E = lg.shape
-    k = selected.shape[-1]
+    T, k = lg.shape[0], selected.shape[-1]
     if selected.shape != (T, k) or d_weights.shape != (T, k) or selected.device != lg.device or d_weights.device != lg.device:
         raise ValueError("selected and d_weights must be [tokens, top_k] tensors on the logits' device")
-    dw = d_weights if d_weights.dtype in (torch.float32, torch.bfloat16) else d_weights.float()
-    dw, sel = dw.contiguous(), selected.to(torch.int64).contiguous()
+    return _router_grouped_backward(lg, selected.to(torch.int64).contiguous(), d_weights, score, renorm, scale)
+
+
+def _router_grouped_backward(lg, sel, d_weights, score, renorm, scale):
+    (T, E), k = lg.shape, sel.shape[1]
+    dw = (d_weights if d_weights.dtype in (torch.float32, torch.bfloat16) else d_weights.float()).contiguous()
     out = _empty((T, E), dtype=lg.dtype, device=lg.device)
     if T == 0:
         return out
