@@ -5,6 +5,10 @@
 //   backward: per piece of the vocabulary, GEMM with the derivative as its epilogue into a bf16 piece [T, piece], then
 //             d W rows of the piece = piece^T h, and fp32 partial sums of d h per segment of 8192 columns, folded in
 //             ascending order. The segments are at absolute positions, so the bits do not depend on the piece width.
+// Bound by the matrix products from some hundred rows on: 16384 rows x 151936 x 2048 take 7.8 ms (1.31 PFLOP/s, 88 % of a
+// library product's rate); 4096 rows with gradients 8.8 ms: forward 1.33, recomputed logits 1.26, d h 1.05, d W 1.08 PFLOP/s
+// (the last two read their operands through 8-byte transposing LDS reads). A few rows are bound by reading the weights once
+// (7 rows: 116 us, 5.7 TB/s).
 #include <algorithm>
 
 #include "gemm_core.h"
