@@ -22,6 +22,7 @@ constexpr int VL_BM = 64, VL_BN = 256, VL_BK = 64;
 constexpr int VL_RB = VL_BK * 2 + 16;  // LDS row pitch: 16 bytes on, so that the rows of a fragment read hit distinct banks
 constexpr int VL_SEG = 8192;           // columns per partial sum of d h
 constexpr int VL_FEW = 64;             // rows up to which the forward streams the weights (gemm_stream_kernel)
+constexpr int VL_ROW_EACH = 512;       // rows up to which the final fold has a workgroup for each
 
 // The general kernel: any H that is a multiple of 8, any number of rows. 64 rows x 256 columns per workgroup, one
 // 64-column strip per wavefront, operands through registers into one of two LDS buffers.
@@ -112,29 +113,38 @@ __global__ __launch_bounds__(256) void vocab_gemm_kernel(GemmParams p) {
 
 // out = x[label] - lse, lse = M + log S over a row's tile statistics. One wavefront per row, lane r folds the tiles r, r + 64,
 // ... in ascending order, then the lanes fold pairwise (r with r ^ 32, then 16, ... 1). STRIPS: the four strips of a tile
-// come one by one. 16 rows per workgroup: with [tile][row] partials one of its loads then uses whole 128-byte lines.
-template <bool STRIPS>
-__global__ __launch_bounds__(1024) void vocab_final_kernel(const float2* __restrict__ part, int64_t part_ld, int ntiles, int nstrips,
+// come one by one. Up to 512 rows a workgroup each and ten tiles of a lane on their way at once, since the time is that of
+// trips to memory (V = 151936: 16 rows 132 -> 116 us the whole call, 300 rows 4 us less); more rows in workgroups of 16: with
+// [tile][row] partials one of its loads then uses whole 128-byte lines (8192 rows x 256: 697 against 737 us).
+template <bool STRIPS, int ROWS>
+__global__ __launch_bounds__(64 * ROWS) void vocab_final_kernel(const float2* __restrict__ part, int64_t part_ld, int ntiles, int nstrips,
                                                            const float* __restrict__ label_logit, const int64_t* __restrict__ labels,
                                                            float* __restrict__ out, float* __restrict__ lse_out, int64_t T, int64_t V) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * ROWS + (threadIdx.x >> 6);
   if (row >= T) return;
   float m = -INFINITY, sum = 0.f;
-#pragma unroll 4
-  for (int t = lane; t < ntiles; t += 64) {
-    float2 a;
-    if constexpr (STRIPS) {
-      float2 st[4];
+  constexpr int U = ROWS == 1 ? 10 : 4, NS = STRIPS ? 4 : 1;
+  const int last = (STRIPS ? nstrips : ntiles) - 1;
+  for (int t0 = lane; t0 < ntiles; t0 += 64 * U) {
+    float2 st[U][NS];
 #pragma unroll
-      for (int j = 0; j < 4; j++) st[j] = 4 * t + j < nstrips ? part[(int64_t)(4 * t + j) * part_ld + row] : make_float2(-INFINITY, 0.f);
-      a = st[0];
+    for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int j = 1; j < 4; j++) vocab_fold(a.x, a.y, st[j].x, st[j].y);
-    } else {
-      a = part[(int64_t)t * part_ld + row];
+      for (int j = 0; j < NS; j++) st[u][j] = part[(int64_t)min(NS * (t0 + 64 * u) + j, last) * part_ld + row];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int t = t0 + 64 * u;
+      if (t < ntiles) {
+        float2 a = st[u][0];
+#pragma unroll
+        for (int j = 1; j < NS; j++) {
+          const bool there = NS * t + j <= last;
+          vocab_fold(a.x, a.y, there ? st[u][j].x : -INFINITY, there ? st[u][j].y : 0.f);
+        }
+        vocab_fold(m, sum, a.x, a.y);
+      }
     }
-    vocab_fold(m, sum, a.x, a.y);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -301,10 +311,14 @@ int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* lab
     const int rc = launch_vocab_gemm<EPI_LSE>(p, T, stream);
     if (rc != VX_OK) return rc;
   }
-  const unsigned grid = (unsigned)((T + 15) / 16);
   const int nstrips = (int)((V + 63) / 64);
-  if (few) vocab_final_kernel<true><<<grid, 1024, 0, stream>>>(p.lse_part, T, (int)ntiles, nstrips, p.label_logit, labels, out, lse, T, V);
-  else vocab_final_kernel<false><<<grid, 1024, 0, stream>>>(p.lse_part, T, (int)ntiles, nstrips, p.label_logit, labels, out, lse, T, V);
+  auto final = [&](auto kernel, int64_t rows) {
+    kernel<<<(unsigned)((T + rows - 1) / rows), 64 * rows, 0, stream>>>(p.lse_part, T, (int)ntiles, nstrips, p.label_logit, labels, out, lse, T, V);
+  };
+  static_assert(VL_FEW <= VL_ROW_EACH);
+  if (few) final(vocab_final_kernel<true, 1>, 1);
+  else if (T <= VL_ROW_EACH) final(vocab_final_kernel<false, 1>, 1);
+  else final(vocab_final_kernel<false, 16>, 16);
   return launch_status();
 }
 
