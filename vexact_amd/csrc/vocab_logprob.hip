@@ -8,7 +8,7 @@
 // Bound by the matrix products from some hundred rows on: 16384 rows x 151936 x 2048 take 7.8 ms (1.31 PFLOP/s, 88 % of a
 // library product's rate); 4096 rows with gradients 8.8 ms: forward 1.33, recomputed logits 1.26, d h 1.05, d W 1.08 PFLOP/s
 // (the last two read their operands through 8-byte transposing LDS reads). A few rows are bound by reading the weights once
-// (7 rows: 116 us, 5.7 TB/s).
+// (7 rows: 114 us, 5.7 TB/s).
 #include <algorithm>
 
 #include "gemm_core.h"
