@@ -155,3 +155,24 @@ def test_second_derivatives_are_refused():
         assert not plain.requires_grad and again.requires_grad
         with pytest.raises(RuntimeError, match="once_differentiable"):
             again.float().sum().backward()
+
+
+@pytest.mark.parametrize("which", ["hidden", "weight", "labels", "logits"])
+def test_operands_changed_before_the_backward_are_noticed(which):
+    """What the backward would read again must not have changed in place; copies that were made on the way may."""
+    g = torch.Generator().manual_seed(6)
+    t = dict(hidden=torch.randn(2, 6, 64, generator=g).to(torch.bfloat16).cuda(), weight=torch.randn(200, 64, generator=g).to(torch.bfloat16).cuda(),
+             labels=torch.randint(0, 200, (2, 6), generator=g).cuda(), logits=torch.randn(12, 32, generator=g).cuda())
+    leaves = {n: t[n].requires_grad_() for n in ("hidden", "weight", "logits")}
+    out = grouped_topk_router(t["logits"], 4)[0] if which == "logits" else logprobs_from_hidden(t["hidden"], t["weight"], t["labels"])
+    with torch.no_grad():
+        t[which].zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.float().sum().backward()
+    # the rows of an expanded hidden state are copied for the kernel: the gradient is that of the call
+    row = t["hidden"].detach()[0, :1].clone().requires_grad_()
+    lp = logprobs_from_hidden(row.expand(6, 64), leaves["weight"].detach(), torch.arange(6).cuda())
+    (want,) = torch.autograd.grad(lp.sum(), row, retain_graph=True)
+    with torch.no_grad():
+        row.zero_()
+    assert_bitwise(torch.autograd.grad(lp.sum(), row)[0], want)

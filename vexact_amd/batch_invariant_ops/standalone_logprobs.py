@@ -46,9 +46,11 @@ class _HiddenLogprobsFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, labels, temperature):
-        x, w, flat_labels, scale = ops._vocab_operands(hidden.reshape(-1, hidden.shape[-1]), weight, labels, temperature)
+        flat = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
+        x, w, flat_labels, scale = ops._vocab_operands(flat, weight, labels, temperature)
         out, lse = ops._vocab_forward(x, w, flat_labels, scale)
-        ctx.save_for_backward(x, w, flat_labels, lse)  # as the kernels take them: nothing to check or copy again
+        # as the kernels take them: nothing to check or copy again
+        ctx.save_for_backward(hidden if x is flat else x, w, flat_labels, lse)
         ctx.scale, ctx.hidden_shape = scale, hidden.shape
         return out.reshape(labels.shape)
 
@@ -56,6 +58,8 @@ class _HiddenLogprobsFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_out):
         x, w, labels, lse = ctx.saved_tensors
+        if x.dim() != 2:
+            x = x.reshape(-1, x.shape[-1])
         need_hidden, need_weight = ctx.needs_input_grad[:2]
         d_hidden, d_weight = ops._vocab_backward(x, w, labels, lse, d_out, ctx.scale, need_hidden, need_weight)
         return d_hidden.reshape(ctx.hidden_shape) if need_hidden else None, d_weight, None, None
