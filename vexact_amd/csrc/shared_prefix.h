@@ -110,7 +110,7 @@ __device__ __forceinline__ SharedGroup shared_group_of(const AttnParams& p, cons
 // engines left half of the CUs without work (16 groups of 16: 138 against 91 us). All 64 lanes call it.
 __device__ __forceinline__ bool shared_block(const AttnParams& p, const SharedParams& s, int item, int rb, SharedGroup& sg, int& place) {
   const int lane = threadIdx.x & 63, G = p.Hq / p.Hkv;
-  int base = 0;  // blocks of the 64 groups at a time before these
+  int base = 0;  // blocks of the groups in front of these 64
   for (int b = 0; b < s.num_groups; b += 64) {
     const SharedLane gl = shared_lane(p, s, b);
     const int mine = gl.n < 2 ? 0 : (int)(((int64_t)gl.n * G + rb - 1) / rb);
