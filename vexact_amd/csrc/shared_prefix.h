@@ -15,7 +15,7 @@
 // images of them, but its steps are a chain, and at 16 groups of 16 it leaves half of the CUs without one: level at 8192
 // query rows, 4 times slower for one group of 64 on 32768 keys.)
 // At a full decode batch both launches run at the rate of a large copy: what they move is the prefixes once (241 MB at 16
-// groups of 16 on prefixes about 7400, 32 / 4 heads), their images twice (2 x 131 MB) and the tails (300 MB): 143 + 37 us.
+// groups of groups of 16 on prefixes about 7400, 32 / 4 heads), their images twice (2 x 131 MB) and the tails (300 MB): 138 + 33 us.
 #pragma once
 #include "attn_core.h"
 
@@ -33,9 +33,9 @@ struct SharedParams {
   float* own_part;
   int64_t own_floats;
   int max_own;
-  int blocks;             // launch 1: row blocks per (chunk, kv head), workgroups of the shared part,
-  int shared_wgs, own_wgs;  // (multiples of 8), of the own part, chunks that a shared workgroup takes,
-  int cpw, splits;         // and workgroups that share the own chunks of one (sequence, kv head)
+  // launch 1: workgroups of the shared part that have work if the prefixes are equally long, of the own part (multiples of
+  // 8), chunks that a shared workgroup takes, workgroups that share the own chunks of one (sequence, kv head)
+  int shared_sure, own_first, own_wgs, cpw, splits;
 };
 
 static inline int64_t shared_image_floats(int64_t rows, int64_t dv) { return (rows * ((dv + 3) / 4 * 4 + 2) + 3) / 4 * 4; }
@@ -104,53 +104,63 @@ __device__ __forceinline__ SharedGroup shared_group_of(const AttnParams& p, cons
   if (seq >= r.seq0 + r.n) r.chunks = 0;
   return r;
 }
-// Which group row block `item` (rb rows) belongs to, and its place there; false behind the last one. The blocks that the
-// groups really have are numbered first: the launch has room for a partly filled block per group, and with the unused
-// ones in between (every other one where each group fills exactly one) the dispatcher's fixed round of the shader
-// engines left half of the CUs without work (16 groups of 16: 138 against 91 us). All 64 lanes call it.
-__device__ __forceinline__ bool shared_block(const AttnParams& p, const SharedParams& s, int item, int rb, SharedGroup& sg, int& place) {
+// Shared workgroup `index` -> its kv head, first chunk and row block (rb rows): the group and the block's place in it; false
+// if there is nothing for it. All 64 lanes call it. An XCD has an L2 of its own: chunk c belongs to XCD c % 8, where all row
+// blocks of a (chunk, kv head) follow each other, so the second row block of a large group finds the chunk's keys in the
+// L2. A workgroup takes cpw chunks, 8 apart. Only the blocks that the groups really have are numbered, so the workgroups
+// that the launch has too many (a partly filled block per group: its host knows no sizes) come last. Between the others
+// they cost a workgroup's slot for three trips to memory, and where every other one is empty (16 groups that fill a block
+// each) the dispatcher's fixed round of the shader engines leaves half of the CUs without work (138 against 91 us).
+__device__ __forceinline__ bool shared_unit(const AttnParams& p, const SharedParams& s, int index, int rb, SharedGroup& sg, int& place, int& kvh, int& chunk) {
   const int lane = threadIdx.x & 63, G = p.Hq / p.Hkv;
-  int base = 0;  // blocks of the groups in front of these 64
-  for (int b = 0; b < s.num_groups; b += 64) {
-    const SharedLane gl = shared_lane(p, s, b);
-    const int mine = gl.n < 2 ? 0 : (int)(((int64_t)gl.n * G + rb - 1) / rb);
-    int end = mine;  // inclusive sum over the lanes
+  SharedLane gl;
+  int mine, end;  // blocks of this lane's group; of this and the lower lanes' groups
+  auto read = [&](int b) {
+    gl = shared_lane(p, s, b);
+    end = mine = gl.n < 2 ? 0 : (int)(((int64_t)gl.n * G + rb - 1) / rb);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int v = __shfl_up(end, o, 64);
       if (lane >= o) end += v;
     }
-    const uint64_t after = __ballot(base + end > item);
-    if (after) {
-      const int l = __builtin_ctzll(after);
-      place = item - base - __builtin_amdgcn_readlane(end - mine, l);
+    return __builtin_amdgcn_readlane(end, 63);
+  };
+  int total = 0;
+  for (int b = 0; b < s.num_groups; b += 64) total += read(b);
+  if (total == 0) return false;
+  const int local = index >> 3, pair = local / total;
+  kvh = pair % p.Hkv;
+  chunk = pair / p.Hkv * (8 * s.cpw) + (index & 7);
+  if (chunk >= s.max_chunks) return false;
+  int item = local - pair * total;
+  for (int b = 0;; b += 64) {
+    const int here = s.num_groups <= 64 ? total : read(b);
+    if (item < here) {
+      const int l = __builtin_ctzll(__ballot(end > item));
+      place = item - __builtin_amdgcn_readlane(end - mine, l);
       sg = shared_group(p, s, gl, l, b + l);
       return true;
     }
-    base += __builtin_amdgcn_readlane(end, 63);
+    item -= here;
   }
-  return false;
 }
 
-// Launch 1 holds shared and own workgroups; returns the index within the kind, -1 - index for an own one. They alternate in
-// proportion, so that a CU runs one that waits for the matrix core beside one that waits for memory (16 groups of 16: 160 ->
-// 153 us); always eight consecutive ids, which go round the eight XCDs, are of one kind.
+// Launch 1 holds shared and own workgroups; returns the index within the kind, -1 - index for an own one. In front are those
+// that surely have work, a block or more per group and the first own workgroup of every pair, alternating in proportion, so
+// that a CU runs one that waits for the matrix core beside one that waits for memory; behind them the further own
+// workgroups, then the rest of the shared ones, most of which have nothing to do (against all of both kinds alternating,
+// with every pair's own workgroups together: 16 groups of 16 175 -> 170 us, 128 sequences in 32 groups 87 -> 68, 45 in 7
+// uneven groups 35 -> 32). Always eight consecutive ids, which go round the eight XCDs, are of one kind.
 __device__ __forceinline__ int shared_kind(const SharedParams& sp) {
-  const int grp = blockIdx.x >> 3;
-  const int64_t own = sp.own_wgs >> 3, all = own + (sp.shared_wgs >> 3);
-  const int before = (int)(grp * own / all), upto = (int)((grp + 1) * own / all);
-  return upto > before ? -1 - (before * 8 + (int)(blockIdx.x & 7)) : (grp - before) * 8 + (int)(blockIdx.x & 7);
+  const int grp = blockIdx.x >> 3, in = blockIdx.x & 7;
+  const int64_t first = sp.own_first >> 3, all = first + (sp.shared_sure >> 3), rest = (sp.own_wgs - sp.own_first) >> 3;
+  if (grp >= all + rest) return (int)(grp - first - rest) * 8 + in;
+  if (grp >= all) return -1 - ((int)(grp - all + first) * 8 + in);
+  const int before = (int)(grp * first / all), upto = (int)((grp + 1) * first / all);
+  return upto > before ? -1 - (before * 8 + in) : (grp - before) * 8 + in;
 }
 
-// Shared workgroup -> (first chunk, kv head, row block). An XCD has an L2 of its own: chunk c belongs to XCD c % 8, where all
-// row blocks of a (chunk, kv head) follow each other, so the second row block of a large group finds the chunk's keys in
-// the L2. A workgroup takes cpw chunks, 8 apart.
-__device__ __forceinline__ void shared_place(const SharedParams& sp, int index, int Hkv, int& block, int& kvh, int& chunk) {
-  const int local = index >> 3;
-  block = local % sp.blocks;
-  kvh = local / sp.blocks % Hkv;
-  chunk = local / sp.blocks / Hkv * (8 * sp.cpw) + (index & 7);
-}
+// workgroups for `blocks` row blocks
 static inline int64_t shared_wgs(int64_t blocks, int Hkv, int chunks, int cpw) { return blocks * Hkv * ((chunks + 8 * cpw - 1) / (8 * cpw) * 8); }
 
 // the state of one 16-row tile in the registers of AttnWave -> an image of `rows` rows (lane r16 = row `row`)
@@ -174,15 +184,15 @@ __device__ __forceinline__ void shared_store(const W& w, int t, float* image, in
 }
 
 // Launch 1, own part: wavefront i of WAVES in workgroup (u, z) takes the own chunks
-// z WAVES + i, + splits WAVES, ... of pair u = (sequence, kv head). A run of pairs goes to one XCD, so that the keys of the
+// z WAVES + i, + splits WAVES, ... of pair u = (sequence, kv head); the first workgroups of all pairs come first. A run of pairs goes to one XCD, so that the keys of the
 // partly shared chunk at a prefix's end come from its L2 for all but the first sequence of a group.
 template <class ET, int DK, int DV, int QT, int KIND, int WAVES, bool PAD>
 __device__ __forceinline__ void attn_own_chunks(const AttnParams& p, const SharedParams& sp, int o) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, r16 = lane & 15;
   const int per = ((int64_t)p.num_seqs * p.Hkv + 7) / 8;  // pairs of an XCD
-  const int local = o >> 3, u = (o & 7) * per + local / sp.splits, z = local % sp.splits;
-  if (local / sp.splits >= per || u >= p.num_seqs * p.Hkv) return;
+  const int local = o >> 3, u = (o & 7) * per + local % per, z = local / per;
+  if (u >= p.num_seqs * p.Hkv) return;
   const int seq = u / p.Hkv, kvh = u % p.Hkv, G = p.Hq / p.Hkv;
   const int q0 = p.cu_q[seq], qlen = p.cu_q[seq + 1] - q0;
   const int kv_len = min(p.seqused_k[seq], p.max_kv);
@@ -220,11 +230,10 @@ __global__ __launch_bounds__(64) void attn_shared_chunks_kernel(AttnParams p, Sh
     attn_own_chunks<ET, DK, DV, QT, KIND, 1, PAD>(p, sp, -1 - index);
     return;
   }
-  int block, kvh, chunk, place;
-  shared_place(sp, index, p.Hkv, block, kvh, chunk);
+  int kvh, chunk, place;
   const int G = p.Hq / p.Hkv;
   SharedGroup sg;
-  if (!shared_block(p, sp, block, 16, sg, place)) return;
+  if (!shared_unit(p, sp, index, 16, sg, place, kvh, chunk)) return;
   const int row0 = place * 16;
   if (chunk >= sg.chunks || row0 >= sg.n * G) return;
   const int r16 = threadIdx.x & 15;
@@ -377,11 +386,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
   }
   constexpr int D = 128, KS = D / 32, RB = 64 * TILES;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * SPL_STAGE];
-  int block, kvh, chunk, place;
-  shared_place(sp, index, p.Hkv, block, kvh, chunk);
+  int kvh, chunk, place;
   const int G = p.Hq / p.Hkv;
   SharedGroup sg;
-  if (!shared_block(p, sp, block, RB, sg, place)) return;
+  if (!shared_unit(p, sp, index, RB, sg, place, kvh, chunk)) return;
   const int rows = sg.n * G, row0 = place * RB;
   if (chunk >= sg.chunks || row0 >= rows) return;  // uniform over the block
   constexpr int nb = ATT_CHUNK / ATT_BLOCK;
@@ -505,19 +513,21 @@ static int launch_shared_prefix_t(const AttnParams& p, SharedParams sp, hipStrea
   constexpr int WAVES = LDS ? 4 : 1;
   // row tiles per wavefront: one where an average group has at most 64 rows, else two
   const int tiles = LDS && rows > 64 * (int64_t)sp.num_groups ? 2 : 1;
-  sp.blocks = (int)(rows / (16 * WAVES * tiles) + sp.num_groups);
+  const int64_t full = std::max<int64_t>(sp.num_groups, rows / (16 * WAVES * tiles)), blocks = rows / (16 * WAVES * tiles) + sp.num_groups;
   // Chunks per workgroup of the LDS form: its set-up (group, block table, queries) costs as much as two chunks, so several
   // where that leaves about 1536 workgroups (64 sequences on 32768 keys: 138 us with one chunk each, 94 with two, 103 with
   // four; 16 groups of 16: 153 / 143 / 143)
-  const int64_t units = (int64_t)sp.blocks * p.Hkv * sp.max_chunks;
+  const int64_t units = blocks * p.Hkv * sp.max_chunks;
   sp.cpw = LDS ? (int)std::max<int64_t>(1, std::min<int64_t>(16, units / 1536)) : 1;
-  const int64_t swgs = sp.num_groups == 0 || sp.max_chunks == 0 ? 0 : shared_wgs(sp.blocks, p.Hkv, sp.max_chunks, sp.cpw);
-  // about 4096 wavefronts for the own chunks, at most one per chunk
-  sp.splits = (int)std::max<int64_t>(1, std::min<int64_t>((sp.max_own + WAVES - 1) / WAVES, 4096 / (pairs * WAVES)));
+  const int64_t swgs = sp.num_groups == 0 || sp.max_chunks == 0 ? 0 : shared_wgs(blocks, p.Hkv, sp.max_chunks, sp.cpw);
+  // about 8192 wavefronts for the own chunks, at most one per chunk (16 groups of 16: 172 / 170 / 170 us with 4096 / 8192 /
+  // 16384, 128 sequences in 32 groups 68 / 68 / 72)
+  sp.splits = (int)std::max<int64_t>(1, std::min<int64_t>((sp.max_own + WAVES - 1) / WAVES, 8192 / (pairs * WAVES)));
   const int64_t owgs = (pairs + 7) / 8 * 8 * sp.splits;
   if (swgs + owgs > 0x7fffffff) return VX_ERR_UNSUPPORTED;
-  sp.shared_wgs = (int)swgs;
+  sp.shared_sure = (int)std::min(swgs, shared_wgs(full, p.Hkv, sp.max_chunks, sp.cpw));
   sp.own_wgs = (int)owgs;
+  sp.own_first = (int)((pairs + 7) / 8 * 8);
   const unsigned grid = (unsigned)(swgs + owgs);
   if constexpr (LDS) {
     if (tiles == 2) attn_shared_chunks_lds_kernel<ET, 2, QT, KIND><<<grid, 256, 0, stream>>>(p, sp);
