@@ -15,7 +15,7 @@
 // images of them, but its steps are a chain, and at 16 groups of 16 it leaves half of the CUs without one: level at 8192
 // query rows, 4 times slower for one group of 64 on 32768 keys.)
 // At a full decode batch both launches run at the rate of a large copy: what they move is the prefixes once (241 MB at 16
-// groups of groups of 16 on prefixes about 7400, 32 / 4 heads), their images twice (2 x 131 MB) and the tails (300 MB): 138 + 33 us.
+// groups of 16 on prefixes about 7400, 32 / 4 heads), their images twice (2 x 131 MB) and the tails (300 MB): 138 + 33 us.
 #pragma once
 #include "attn_core.h"
 
