@@ -203,6 +203,31 @@ def test_padded_batches():
 
 @gpu
 @pytest.mark.parametrize("heads,dims,page", [((8, 2), (128, 128), 16), ((6, 2), (64, 64), 16), ((4, 4), (80, 80), 24)])
+def test_an_ended_sequence_inside_a_group(heads, dims, page):
+    """A slot without a query token keeps the length of the sequence that ended in it, the longest of its group, and a block
+    table whose (valid) pages hold other keys by now. The others' prefix is read from one of their own tables, and is
+    shared no further than one of them reaches."""
+    a = make([4, 3], [960, 960], [120, 300, 40], heads, dims, page, seed=13)
+    table, used = a["page_table"].clone(), a["seqused_k"].clone()
+    pages = torch.arange(a["k_cache"].shape[0] - 1, -1, -1, dtype=torch.int32).cuda()
+    gone = (1, 4)
+    for s in gone:
+        n = int((table[s] < (1 << 30)).sum())
+        assert not torch.equal(table[s, :n], pages[:n])
+        table[s, :n] = pages[:n]
+        used[s] = n * page
+    used[5], used[6] = 700, 530  # of the second group nobody else reaches the prefix's end
+    assert int(used[:4].argmax()) == 1 and int(used[4:].argmax()) == 0
+    cu = [0]
+    for s in range(7):
+        cu.append(cu[-1] + (s not in gone))
+    a.update(page_table=table, seqused_k=used, cu_seqlens_q=torch.tensor(cu, dtype=torch.int32).cuda(), q=a["q"][: cu[-1]].contiguous())
+    out = ops.shared_prefix_attention(**a)
+    assert_bitwise(out, paged(a, decode_kernel="split"))
+
+
+@gpu
+@pytest.mark.parametrize("heads,dims,page", [((8, 2), (128, 128), 16), ((6, 2), (64, 64), 16), ((4, 4), (80, 80), 24)])
 def test_what_lies_behind_a_short_sequence_inside_the_prefix(heads, dims, page):
     """Sequences that end inside their group's prefix read nothing of the keys behind their end, which for them may hold
     anything, though others of the group do: infinite keys, NaN and infinite values."""

@@ -44,7 +44,7 @@ struct SharedGroup {
   int seq0, n;  // first sequence, how many
   int tile0;    // first 16-row tile of the group in the workspace
   int chunks;   // whole chunks of keys that are computed once for the group
-  int src;      // a sequence of the group that holds all of them: its block table is read
+  int src;      // a sequence of the group, with a query token, that holds all of them: its block table is read
 };
 // The offsets and prefix lengths of 64 groups from `b` on, one per lane, so that whichever is wanted needs no second round
 // trip to memory.
@@ -63,7 +63,8 @@ __device__ __forceinline__ SharedLane shared_lane(const AttnParams& p, const Sha
   return l;
 }
 // The group in lane `from` of l (group g). All 64 lanes call it. The shared keys end where the longest sequence of the
-// group ends, whatever prefix_len says, so that the block table that is read covers them.
+// group ends, whatever prefix_len says, so that the block table that is read covers them. A slot without a query token
+// counts as empty: its length and block table may be those of a sequence that has ended, its pages another's by now.
 __device__ __forceinline__ SharedGroup shared_group(const AttnParams& p, const SharedParams& s, const SharedLane& l, int from, int g) {
   const int lane = threadIdx.x & 63;
   SharedGroup r;
@@ -73,7 +74,11 @@ __device__ __forceinline__ SharedGroup shared_group(const AttnParams& p, const S
   int longest = 0;
   r.src = r.seq0;
   for (int b = 0; b < r.n; b += 64) {
-    const int len = b + lane < r.n ? min(p.seqused_k[r.seq0 + b + lane], p.max_kv) : 0;
+    int len = 0;
+    if (b + lane < r.n) {
+      const int i = r.seq0 + b + lane, used = min(p.seqused_k[i], p.max_kv);
+      len = p.cu_q[i + 1] > p.cu_q[i] ? used : 0;
+    }
     int m = len;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
