@@ -110,7 +110,8 @@ int vx_logprobs_static(const void* logits, const int64_t* labels, float* out, in
  * multiples of 4, either may be null), from the forward's lse and d_out [T] fp32. Rows whose label is outside the
  * vocabulary have no gradient and leave none in d_weight, whatever they and their d_out hold. The derivative of each
  * logit is rounded to bf16 once before the two products, which accumulate in fp32; no atomics, results repeat bit for bit. T <= 2^32 / 16384 rows.
- * H and row pitches up to 2^22 elements; the backward takes a weight pitch below 2^18. */
+ * H up to 2^22, row pitches of hidden and weight 0 (one row for all) to 2^22 elements; the backward takes a weight pitch
+ * below 2^18. */
 int64_t vx_vocab_logprobs_workspace_bytes(int64_t T, int64_t V);
 int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* labels, float* out, float* lse, int64_t T,
                       int64_t V, int64_t H, int64_t ldh, int64_t ldw, float scale, void* workspace,

@@ -344,3 +344,47 @@ def test_c_abi_refuses_rows_too_far_apart():
     for H, ldh, ldw in ((16, 1 << 23, 16), (16, 16, 1 << 23), (16, 1 << 40, 16), (16, 16, 1 << 40), (1 << 23, 1 << 23, 1 << 23), (16, -16, 16), (16, 16, -16)):
         assert lib.vx_vocab_logprobs(a, a, a, a, a, 4, 10, H, ldh, ldw, 1.0, a, 1 << 40, None) == -2
         assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, 4, 10, H, ldh, ldw, H, H, 1.0, a, 1 << 60, None) == -2
+
+
+def _entries(h, ldh, w, ldw, y, d, T, V, H):
+    """The C entry points, with row pitches that no tensor of the front end has: (out, lse, d_hidden, d_weight)."""
+    from vexact_amd import _lib
+
+    lib = _lib.load()
+    f = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device="cuda")  # noqa: E731
+    out, lse, dh, dw = f(T), f(T), f(T, H, dtype=torch.bfloat16), f(V, H, dtype=torch.bfloat16)
+    ws = f(max(lib.vx_vocab_logprobs_workspace_bytes(T, V), lib.vx_vocab_logprobs_bwd_workspace_bytes(T, V, H)), dtype=torch.uint8)
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(lib.vx_vocab_logprobs(h.data_ptr(), w.data_ptr(), y.data_ptr(), out.data_ptr(), lse.data_ptr(), T, V, H, ldh, ldw, 1.0,
+                                     ws.data_ptr(), ws.numel(), stream), "forward")
+    _lib.check(lib.vx_vocab_logprobs_bwd(h.data_ptr(), w.data_ptr(), y.data_ptr(), lse.data_ptr(), d.data_ptr(), dh.data_ptr(), dw.data_ptr(),
+                                         T, V, H, ldh, ldw, H, H, 1.0, ws.data_ptr(), ws.numel(), stream), "backward")
+    return out, lse, dh, dw
+
+
+@gpu
+@pytest.mark.parametrize("T,V,H", [(5, 70, 64), (300, 9000, 128), (70, 300, 72)])
+def test_one_row_for_all(T, V, H):
+    """A row pitch of zero, of the hidden states and of the weights: the values of copies of that row."""
+    h, w, y = (t.cuda() for t in make(T, V, H, seed=31))
+    d = torch.linspace(-1, 1, T).cuda()
+    h1, w1 = h[:1].expand(T, H).contiguous(), w[:1].expand(V, H).contiguous()
+    for got, want in ((_entries(h, 0, w, H, y, d, T, V, H), _entries(h1, H, w, H, y, d, T, V, H)),
+                      (_entries(h, H, w, 0, y, d, T, V, H), _entries(h, H, w1, H, y, d, T, V, H))):
+        for a, b in zip(got, want):
+            assert_bitwise(a, b)
+
+
+def test_c_abi_zero_row_pitch():
+    """The plan of the backward's pieces does not divide by a row pitch of zero (no GPU needed: the workspace is too small)."""
+    from vexact_amd import _lib
+
+    lib, a = _lib.load(), 4096
+    for ldh, ldw in ((16, 0), (0, 16), (0, 0), (16, 8)):
+        assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, 4, 10, 16, ldh, ldw, 16, 16, 1.0, a, 16, None) == -3
+    # what the workspace function promises is enough whatever the pitch, also where a row's length splits the vocabulary
+    T, V, H = 4, 1 << 20, 1 << 17
+    n = lib.vx_vocab_logprobs_bwd_workspace_bytes(T, V, H)
+    for ldw in (0, 8, H, H + 8):
+        assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, T, V, H, H, ldw, H, H, 1.0, a + 8, n, None) == -3  # misaligned, after the plan
+        assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, T, V, H, H, ldw, H, H, 1.0, a, n // 2, None) == -3

@@ -333,7 +333,7 @@ int vx_vocab_logprobs_bwd(const void* hidden, const void* weight, const int64_t*
   if (!hidden || !weight || !labels || !lse || !d_out || (!d_hidden && !d_weight) || T <= 0 || V <= 0 || H <= 0) return VX_ERR_ARG;
   if (!vocab_args_ok(hidden, weight, T, V, H, ldh, ldw)) return VX_ERR_UNSUPPORTED;
   if ((d_hidden && (ld_dh % 4 || ((uintptr_t)d_hidden & 7))) || (d_weight && (ld_dw % 4 || ((uintptr_t)d_weight & 7)))) return VX_ERR_UNSUPPORTED;
-  const VocabPlan q = vocab_plan(T, V, H, ldw);
+  const VocabPlan q = vocab_plan(T, V, H, std::max(ldw, H));  // rows closer than H, or one for all: as vx_vocab_logprobs_bwd_workspace_bytes plans
   const int64_t lim = (int64_t)1 << 32;
   if ((T * q.ld + VL_SEG) * 2 >= lim || (q.per * VL_SEG * ldw + H) * 2 >= lim || (T * H / 4 + 255) / 256 > 0x7fffffff) return VX_ERR_UNSUPPORTED;
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < q.bytes()) return VX_ERR_WORKSPACE;
