@@ -100,7 +100,7 @@ int vx_logprobs_static(const void* logits, const int64_t* labels, float* out, in
                        int64_t rows, int64_t n, int64_t x_stride, hipStream_t stream);
 
 /* Log-probabilities of given tokens from the hidden states [T, H] and the output projection [V, H] (both bf16, H
- * contiguous, H a multiple of 8, 16-byte aligned rows): x = scale * hidden weight^T (scale = 1 / temperature) in fp32,
+ * contiguous, H a multiple of 8, 16-byte aligned rows): x = scale * hidden weight^T (scale = 1 / temperature, 2^-126 to 2^127) in fp32,
  * lse = logsumexp(x), out[i] = x[i, labels[i]] - lse[i]; neither the logits nor a rounded copy of them reaches memory.
  * out and lse [T] fp32, either may be null. A label outside [0, V) gives NaN (as vx_logprobs). The fold over the
  * vocabulary is at fixed positions: a row's bits do not depend on T. They are not the bits of vx_logprobs on a bf16

@@ -388,3 +388,38 @@ def test_c_abi_zero_row_pitch():
     for ldw in (0, 8, H, H + 8):
         assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, T, V, H, H, ldw, H, H, 1.0, a + 8, n, None) == -3  # misaligned, after the plan
         assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, T, V, H, H, ldw, H, H, 1.0, a, n // 2, None) == -3
+
+
+@gpu
+def test_temperatures():
+    """Those whose reciprocal fp32 does not hold are refused; at the largest allowed the distribution is uniform, whether or not
+    the vocabulary ends inside a tile; at a small one the largest logit takes it all."""
+    for V in (500, 512, 64):
+        h, w, y = make(70, V, 64, seed=33)
+        for bad in (float("inf"), 2.0**127, 2.0**-128, 1e-45, 5e-324, -float("inf")):
+            with pytest.raises(ValueError, match="temperature"):
+                ops.vocab_logprobs(h.cuda(), w.cuda(), y.cuda(), bad)
+            with pytest.raises(ValueError, match="temperature"):
+                logprobs_from_hidden(h.cuda().requires_grad_(), w.cuda(), y.cuda(), bad)
+        for rows in (7, 70):
+            out, lse = ops.vocab_logprobs(h[:rows].cuda(), w.cuda(), y[:rows].cuda(), 2.0**126)
+            # logits below 2^-120, exponentials of 1, an exact sum: one step of a base-2 logarithm in [8, 16) (2^-20, times
+            # log 2), half a step of its product with log 2 (2^-22) and that constant's own rounding (2^-21) are left
+            want = torch.log(torch.tensor(float(V), dtype=torch.float64))
+            assert ((lse.cpu().double() - want).abs() <= 2.0**-19).all() and ((out.cpu().double() + want).abs() <= 2.0**-19).all()
+            best = (h[:rows].double() @ w.double().t()).topk(2, 1)
+            sure = best.values[:, 0] - best.values[:, 1] > 1e-3  # times 2^20: nothing is left of the others
+            out, _ = ops.vocab_logprobs(h[:rows].cuda(), w.cuda(), best.indices[:, 0].cuda(), 2.0**-20)
+            # 0 up to the rounding of the scaled maximum
+            assert sure.any() and (out.cpu().double().abs() <= 2.0**-23 * 2.0**20 * best.values[:, 0].abs())[sure].all()
+
+
+def test_c_abi_refuses_scales_out_of_range():
+    from vexact_amd import _lib
+
+    lib, a = _lib.load(), 4096
+    for scale in (0.0, -1.0, float("inf"), float("nan"), 1e-39, 2.0**127 * 1.5):
+        assert lib.vx_vocab_logprobs(a, a, a, a, a, 4, 10, 16, 16, 16, scale, a, 16, None) == -1
+        assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, 4, 10, 16, 16, 16, 16, 16, scale, a, 16, None) == -1
+    for scale in (2.0**-126, 2.0**127):
+        assert lib.vx_vocab_logprobs(a, a, a, a, a, 4, 10, 16, 16, 16, scale, a, 16, None) == -3

@@ -244,6 +244,10 @@ static bool vocab_args_ok(const void* h, const void* w, int64_t T, int64_t V, in
          gemm_fast_ok(h, w, H, ldh, ldw);
 }
 
+// The kernels work with scale log2 e: an infinite one, or one that the hardware flushes to zero, makes NaN of the -inf that
+// stands in for columns past the vocabulary; a negative one takes the smallest logit for the largest.
+static bool vocab_scale_ok(float scale) { return scale >= 0x1p-126f && scale <= 0x1p127f; }
+
 // columns of one launch: whole 256-column tiles, weight bytes within 32 bits
 static int64_t vocab_cols_limit(int64_t V, int64_t H, int64_t ldw) {
   int64_t n = (V + 255) / 256 * 256;
@@ -292,7 +296,7 @@ int64_t vx_vocab_logprobs_workspace_bytes(int64_t T, int64_t V) {
 
 int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* labels, float* out, float* lse, int64_t T, int64_t V,
                       int64_t H, int64_t ldh, int64_t ldw, float scale, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  if (!hidden || !weight || !labels || (!out && !lse) || T < 0 || V <= 0 || H <= 0) return VX_ERR_ARG;
+  if (!hidden || !weight || !labels || (!out && !lse) || T < 0 || V <= 0 || H <= 0 || !vocab_scale_ok(scale)) return VX_ERR_ARG;
   if (!vocab_args_ok(hidden, weight, T, V, H, ldh, ldw)) return VX_ERR_UNSUPPORTED;
   if (T == 0) return VX_OK;
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < vx_vocab_logprobs_workspace_bytes(T, V)) return VX_ERR_WORKSPACE;
@@ -330,7 +334,8 @@ int64_t vx_vocab_logprobs_bwd_workspace_bytes(int64_t T, int64_t V, int64_t H) {
 int vx_vocab_logprobs_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* lse, const float* d_out,
                           void* d_hidden, void* d_weight, int64_t T, int64_t V, int64_t H, int64_t ldh, int64_t ldw, int64_t ld_dh,
                           int64_t ld_dw, float scale, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  if (!hidden || !weight || !labels || !lse || !d_out || (!d_hidden && !d_weight) || T <= 0 || V <= 0 || H <= 0) return VX_ERR_ARG;
+  if (!hidden || !weight || !labels || !lse || !d_out || (!d_hidden && !d_weight) || T <= 0 || V <= 0 || H <= 0 || !vocab_scale_ok(scale))
+    return VX_ERR_ARG;
   if (!vocab_args_ok(hidden, weight, T, V, H, ldh, ldw)) return VX_ERR_UNSUPPORTED;
   if ((d_hidden && (ld_dh % 4 || ((uintptr_t)d_hidden & 7))) || (d_weight && (ld_dw % 4 || ((uintptr_t)d_weight & 7)))) return VX_ERR_UNSUPPORTED;
   const VocabPlan q = vocab_plan(T, V, H, std::max(ldw, H));  // rows closer than H, or one for all: as vx_vocab_logprobs_bwd_workspace_bytes plans

@@ -290,8 +290,8 @@ def _vocab_operands(hidden, weight, labels, temperature):
         raise ValueError("vocab_logprobs: labels must be integers, one per row of hidden")
     if weight.device != hidden.device or labels.device != hidden.device:
         raise ValueError("vocab_logprobs: hidden, weight and labels must be on one device")
-    if not temperature > 0:
-        raise ValueError("vocab_logprobs: temperature must be positive")
+    if not 2.0**-127 <= temperature <= 2.0**126:
+        raise ValueError(f"vocab_logprobs: temperature must be positive, with a reciprocal that fp32 holds (2^-127 to 2^126), got {temperature}")
     if hidden.shape[1] % 8 or weight.shape[0] == 0:
         raise ValueError(f"vocab_logprobs: H must be a multiple of 8 and V positive, got H = {hidden.shape[1]}, V = {weight.shape[0]}")
     # rows further apart than this put a piece of the vocabulary beyond the kernels' 32-bit offsets
@@ -302,7 +302,7 @@ def _vocab_operands(hidden, weight, labels, temperature):
 
 def vocab_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0):
     """``(logprobs [T], lse [T])`` in fp32 of the tokens ``labels [T]`` under the logits ``hidden [T, H] @ weight [V, H].T /
-    temperature`` (bf16 operands, H a multiple of 8), which never reach memory. A label outside ``[0, V)`` gives NaN. A
+    temperature`` (bf16 operands, H a multiple of 8, temperature 2^-127 to 2^126), which never reach memory. A label outside ``[0, V)`` gives NaN. A
     row's bits depend on its own hidden state only; the logits are not rounded to bf16 as those of ``matmul`` are, so
     they are not the bits of ``logprobs(matmul(...))``."""
     return _vocab_forward(*_vocab_operands(hidden, weight, labels, temperature))
