@@ -310,6 +310,43 @@ def test_attention_wrapper_with_prefix_groups():
     assert_bitwise(outs[1], outs[0])
 
 
+@gpu
+@pytest.mark.parametrize("form", ["fp32", "strided metadata", "default scale", "tensor scale", "under autograd"])
+def test_prefix_groups_refuse_nothing_that_runs_without_them(form):
+    """A context with prefix groups gives what the same context without them gives: the same bits, or the same error."""
+    from types import SimpleNamespace
+
+    from vexact_amd.batch_invariant_ops import flash_attention_forward
+    from vexact_amd.batch_invariant_ops.kv_cache_context import PrefixGroups, clear_kv_cache_context, set_kv_cache_context
+
+    a = make([3, 2], [300, 600], [40, 7], (8, 2), (64, 64), 16, seed=14)
+    table, used, cu = a["page_table"], a["seqused_k"], a["cu_seqlens_q"]
+    q, k, v, scale = a["q"], a["k_cache"], a["v_cache"], 0.1
+    if form == "fp32":
+        q, k, v = q.float(), k.float(), v.float()
+    elif form == "strided metadata":
+        used, cu = torch.stack([used, used], 1)[:, 0], torch.stack([cu, cu], 1)[:, 1]
+        table = table.t().contiguous().t()
+        assert table.stride(-1) != 1 and used.stride(0) == cu.stride(0) == 2
+    elif form != "under autograd":
+        scale = None if form == "default scale" else torch.tensor(0.1)
+    results = []
+    for groups in (None, PrefixGroups(a["group_offsets"], a["prefix_lens"], 600)):
+        set_kv_cache_context(is_paged_attn=True, key_cache={0: k}, value_cache={0: v}, block_tables=table, context_lens=used,
+                             slot_mapping=None, query_start_loc=cu, max_seqlen_q=1, prefix_groups=groups)
+        try:
+            with torch.set_grad_enabled(form == "under autograd"):
+                results.append(flash_attention_forward(SimpleNamespace(layer_idx=0), q.transpose(0, 1).unsqueeze(0), None, None, None, scale)[0])
+        except ValueError as e:
+            results.append(str(e))
+        finally:
+            clear_kv_cache_context()
+    if form == "tensor scale":
+        assert results[0] == results[1] and "softmax_scale" in results[0]
+    else:
+        assert_bitwise(results[1], results[0])
+
+
 def test_refusals():
     z = torch.zeros
     with pytest.raises(ValueError, match="CUDA tensor"):

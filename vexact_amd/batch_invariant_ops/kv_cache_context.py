@@ -47,8 +47,8 @@ class KVCacheContext:
 
     ``block_tables [B, max_blocks]`` int32 (-1 padded), ``slot_mapping [T]`` int32 (-1 = do not
     store), ``context_lens [B]`` int32 (past + new tokens), ``query_start_loc [B+1]`` int32,
-    ``max_seqlen_q`` host int. ``prefix_groups``: a decode step (``max_seqlen_q == 1``) then reads every shared prefix
-    once per group, with the same bits.
+    ``max_seqlen_q`` host int. ``prefix_groups``: a decode step (``max_seqlen_q == 1``) of a bf16 or fp16 model then reads every
+    shared prefix once per group, with the same bits; any other step runs as it does without them.
     """
 
     is_paged_attn: bool = False
