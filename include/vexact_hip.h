@@ -109,9 +109,10 @@ int vx_logprobs_static(const void* logits, const int64_t* labels, float* out, in
  * The backward recomputes x in pieces of the vocabulary: d_hidden [T, H] and / or d_weight [V, H] (bf16, row strides
  * multiples of 4, either may be null), from the forward's lse and d_out [T] fp32. Rows whose label is outside the
  * vocabulary have no gradient and leave none in d_weight, whatever they and their d_out hold. The derivative of each
- * logit is rounded to bf16 once before the two products, which accumulate in fp32; no atomics, results repeat bit for bit. T <= 2^32 / 16384 rows.
- * H up to 2^22, row pitches of hidden and weight 0 (one row for all) to 2^22 elements; the backward takes a weight pitch
- * below 2^18. */
+ * logit is rounded to bf16 once before the two products, which accumulate in fp32; no atomics, results repeat bit for
+ * bit. H up to 2^22, row pitches of hidden and weight 0 (one row for all) to 2^22 elements. The backward takes
+ * T * min(8192, V rounded up to 64) < 2^31 - 8192 (262142 rows from V = 8129 on), 8192 max(ldw, H) + H < 2^31 and
+ * T H < 2^41; its workspace function returns 0 for sizes that it does not take (with ldw <= H). */
 int64_t vx_vocab_logprobs_workspace_bytes(int64_t T, int64_t V);
 int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* labels, float* out, float* lse, int64_t T,
                       int64_t V, int64_t H, int64_t ldh, int64_t ldw, float scale, void* workspace,

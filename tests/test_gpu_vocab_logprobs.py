@@ -423,3 +423,49 @@ def test_c_abi_refuses_scales_out_of_range():
         assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, 4, 10, 16, 16, 16, 16, 16, scale, a, 16, None) == -1
     for scale in (2.0**-126, 2.0**127):
         assert lib.vx_vocab_logprobs(a, a, a, a, a, 4, 10, 16, 16, 16, scale, a, 16, None) == -3
+
+
+def test_c_abi_backward_limits():
+    """The workspace function says which sizes the backward takes, and the backward agrees."""
+    from vexact_amd import _lib
+
+    lib, a = _lib.load(), 4096
+
+    def bwd(T, V, H):  # a workspace that is too small is noticed after the sizes
+        return lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, T, V, H, H, H, H, H, 1.0, a, 16, None)
+
+    for T, V, H in ((262142, 8129, 64), (262142, 151936, 2048), (264000, 8128, 64), (4, 10, 262112), (33554303, 64, 8)):
+        assert lib.vx_vocab_logprobs_bwd_workspace_bytes(T, V, H) > 0 and bwd(T, V, H) == -3, (T, V, H)
+    for T, V, H in ((262143, 8129, 64), (262143, 151936, 2048), (4, 10, 262120), (33554304, 64, 8), (33554303, 64, 1 << 17), (1 << 40, 64, 8)):
+        assert lib.vx_vocab_logprobs_bwd_workspace_bytes(T, V, H) == 0 and bwd(T, V, H) == -2, (T, V, H)
+
+
+@gpu
+def test_most_rows():
+    """As many rows as the backward takes, offsets up to 2^32; one more is refused by the differentiable forward already."""
+    T, V, H = 262142, 8200, 256
+    g = torch.Generator(device="cuda").manual_seed(2)
+    h = torch.randn(T, H, generator=g, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(V, H, generator=g, device="cuda", dtype=torch.bfloat16) * 0.1
+    y = torch.randint(0, V, (T,), generator=g, device="cuda")
+    d = torch.randn(T, generator=g, device="cuda")
+    out, lse = ops.vocab_logprobs(h, w, y)
+    dh, dw = ops.vocab_logprobs_backward(h, w, y, lse, d)
+    for a, b in ((0, 100), (131000, 131100), (T - 100, T)):
+        few, lse_few = ops.vocab_logprobs(h[a:b], w, y[a:b])
+        assert_bitwise(few, out[a:b])
+        assert_bitwise(ops.vocab_logprobs_backward(h[a:b], w, y[a:b], lse_few, d[a:b], need_weight=False)[0], dh[a:b], f"d_hidden of {a}..{b}")
+    for v in (0, 4097, 8191, V - 1):
+        dx = -torch.exp(h.double() @ w[v].double() - lse.double()) * d.double() + torch.where(y == v, d.double(), 0.0)
+        ref, mass = dx @ h.double(), dx.abs() @ h.double().abs()
+        # a half step of each derivative and of the result; 8 sqrt(T) 2^-24 = 2^-12 of the mass for the fp32 sum and 2^-13
+        # for the exponent's argument
+        assert ((dw[v].double() - ref).abs() <= (2.0**-8 + 2.0**-11) * mass + 2.0**-8 * ref.abs()).all()
+    h = torch.zeros(262143, 8, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    w, y = torch.zeros(8192, 8, dtype=torch.bfloat16, device="cuda"), torch.zeros(262143, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="for the backward"):
+        logprobs_from_hidden(h, w, y)
+    with torch.no_grad():  # the forward alone takes it
+        assert ((logprobs_from_hidden(h, w, y) + torch.log(torch.tensor(8192.0))).abs() <= 2.0**-18).all()
+    with pytest.raises(ValueError, match="for the backward"):
+        ops.vocab_logprobs_backward(h, w, y, torch.zeros(262143, device="cuda"), torch.zeros(262143, device="cuda"))

@@ -48,6 +48,7 @@ class _HiddenLogprobsFunction(torch.autograd.Function):
     def forward(ctx, hidden, weight, labels, temperature):
         flat = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
         x, w, flat_labels, scale = ops._vocab_operands(flat, weight, labels, temperature)
+        ops._vocab_backward_bytes(x, w)  # what the backward does not take is refused before it is needed
         out, lse = ops._vocab_forward(x, w, flat_labels, scale)
         # as the kernels take them: nothing to check or copy again
         ctx.save_for_backward(hidden if x is flat else x, w, flat_labels, lse)

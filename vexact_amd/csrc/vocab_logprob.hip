@@ -282,6 +282,12 @@ static VocabPlan vocab_plan(int64_t T, int64_t V, int64_t H, int64_t ldw) {
   return q;
 }
 
+// whether the products over a piece stay within their kernels' 32-bit offsets and grids
+static bool vocab_plan_fits(const VocabPlan& q, int64_t T, int64_t H, int64_t ldw) {
+  const int64_t lim = (int64_t)1 << 32;
+  return (T * q.ld + VL_SEG) * 2 < lim && (q.per * VL_SEG * ldw + H) * 2 < lim && (T * H / 4 + 255) / 256 <= 0x7fffffff;
+}
+
 }  // namespace vx
 
 using namespace vx;
@@ -327,8 +333,9 @@ int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* lab
 }
 
 int64_t vx_vocab_logprobs_bwd_workspace_bytes(int64_t T, int64_t V, int64_t H) {
-  if (T <= 0 || V <= 0 || H <= 0) return 0;
-  return vocab_plan(T, V, H, H).bytes();  // a larger row pitch only makes for more, smaller pieces
+  if (T <= 0 || V <= 0 || H <= 0 || T > 0x7fffff00 || V > 0x7fffff00 || H > VL_MAX_LD) return 0;
+  const VocabPlan q = vocab_plan(T, V, H, H);  // a larger row pitch only makes for more, smaller pieces
+  return vocab_plan_fits(q, T, H, H) ? q.bytes() : 0;
 }
 
 int vx_vocab_logprobs_bwd(const void* hidden, const void* weight, const int64_t* labels, const float* lse, const float* d_out,
@@ -338,9 +345,9 @@ int vx_vocab_logprobs_bwd(const void* hidden, const void* weight, const int64_t*
     return VX_ERR_ARG;
   if (!vocab_args_ok(hidden, weight, T, V, H, ldh, ldw)) return VX_ERR_UNSUPPORTED;
   if ((d_hidden && (ld_dh % 4 || ((uintptr_t)d_hidden & 7))) || (d_weight && (ld_dw % 4 || ((uintptr_t)d_weight & 7)))) return VX_ERR_UNSUPPORTED;
-  const VocabPlan q = vocab_plan(T, V, H, std::max(ldw, H));  // rows closer than H, or one for all: as vx_vocab_logprobs_bwd_workspace_bytes plans
-  const int64_t lim = (int64_t)1 << 32;
-  if ((T * q.ld + VL_SEG) * 2 >= lim || (q.per * VL_SEG * ldw + H) * 2 >= lim || (T * H / 4 + 255) / 256 > 0x7fffffff) return VX_ERR_UNSUPPORTED;
+  // rows closer than H, or one for all: as vx_vocab_logprobs_bwd_workspace_bytes plans
+  const VocabPlan q = vocab_plan(T, V, H, std::max(ldw, H));
+  if (!vocab_plan_fits(q, T, H, std::max(ldw, H))) return VX_ERR_UNSUPPORTED;
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < q.bytes()) return VX_ERR_WORKSPACE;
   bf16_t* dlog = (bf16_t*)workspace;
   float* part = (float*)((uint8_t*)workspace + q.dlog_bytes);

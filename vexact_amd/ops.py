@@ -329,12 +329,23 @@ def vocab_logprobs_backward(hidden: torch.Tensor, weight: torch.Tensor, labels: 
                             d_out: torch.Tensor, temperature: float = 1.0, *, need_hidden: bool = True, need_weight: bool = True):
     """``(d_hidden, d_weight)`` (bf16, None where not needed) of ``vocab_logprobs(hidden, weight, labels, temperature)[0]``
     given its ``lse`` and the incoming ``d_out [T]``. The logits are computed again in pieces of the vocabulary; rows
-    without a valid label have no gradient and leave none in ``d_weight``, whatever they hold."""
+    without a valid label have no gradient and leave none in ``d_weight``, whatever they hold. From V = 8129 on at most
+    262142 rows per call."""
     x, w, lab, scale = _vocab_operands(hidden, weight, labels, temperature)
     T = x.shape[0]
     if lse.dtype != torch.float32 or lse.numel() != T or d_out.numel() != T or lse.device != x.device or d_out.device != x.device:
         raise ValueError("vocab_logprobs: lse (fp32, the forward's) and d_out must have one entry per row, on the rows' device")
     return _vocab_backward(x, w, lab, lse.reshape(-1).contiguous(), d_out, scale, need_hidden, need_weight)
+
+
+def _vocab_backward_bytes(x, w) -> int:
+    """The backward's workspace; raises for sizes that it does not take."""
+    (T, H), V = x.shape, w.shape[0]
+    nbytes = _lib.load().vx_vocab_logprobs_bwd_workspace_bytes(T, V, H)
+    if nbytes == 0 and T > 0:
+        raise ValueError(f"vocab_logprobs: T * min(8192, V rounded up to 64) must be below 2^31 - 8192, 8193 H below 2^31 and T H below 2^41 "
+                         f"for the backward, got T = {T}, V = {V}, H = {H}")
+    return nbytes
 
 
 def _vocab_backward(x, w, lab, lse, d_out, scale, need_hidden, need_weight):
@@ -344,9 +355,10 @@ def _vocab_backward(x, w, lab, lse, d_out, scale, need_hidden, need_weight):
     if T == 0 or not (need_hidden or need_weight):
         return d_x, d_w.zero_() if need_weight else None
     g = d_out.reshape(-1).float().contiguous()
+    nbytes = _vocab_backward_bytes(x, w)
     lib = _lib.load()
     with _on_device(x):
-        ws = _workspace(lib.vx_vocab_logprobs_bwd_workspace_bytes(T, V, H), x.device)
+        ws = _workspace(nbytes, x.device)
         _lib.check(
             lib.vx_vocab_logprobs_bwd(x.data_ptr(), w.data_ptr(), lab.data_ptr(), lse.data_ptr(), g.data_ptr(), _ptr(d_x), _ptr(d_w),
                                       T, V, H, x.stride(0), w.stride(0), H, H, scale, ws.data_ptr(), ws.numel(), _raw_stream(x)),
