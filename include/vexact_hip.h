@@ -265,7 +265,8 @@ int vx_attention_typed(const void* q, const void* k, const void* v, void* out, f
  * rows of out that belong to no sequence, or to one without a query token, are left as they were. max_prefix_len: an upper
  * bound of prefix_lens that sizes the launch and the workspace (longer prefixes are shared up to it). bf16 (dtype 0) or
  * fp16 (1), head sizes up to 256, Hq / Hkv <= 32, caches as for vx_attention. The workspace holds the chunk states
- * (max_kv_len: max_pages * page_size). The reference has no counterpart. */
+ * (max_kv_len: max_pages * page_size); its function returns 0 for sizes that are not supported. The reference has no
+ * counterpart. */
 int64_t vx_shared_prefix_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t Hq, int64_t Hkv, int64_t Dv,
                                          int64_t max_prefix_len, int64_t max_kv_len);
 int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void* out, const int* cu_seqlens_q,

@@ -394,3 +394,20 @@ def test_c_abi_refusals():
     assert lib.vx_shared_prefix_workspace_bytes(4, 2, 8, 2, 128, 512, 700) == (3 * 2 * 2 * 16 + 4 * 2 * 3 * 4) * 130 * 4
     assert lib.vx_shared_prefix_workspace_bytes(4, 2, 8, 2, 128, 255, 256) == 4 * 2 * 4 * 130 * 4
     assert lib.vx_shared_prefix_workspace_bytes(4, 2, 3, 1, 1, 0, 1) == 4 * 20 * 4  # rounded up to 16 bytes
+
+
+def test_c_abi_refuses_sizes_whose_products_wrap():
+    """Counts whose product passes 64 bits (to 0, or below it) are refused like those of a smaller product."""
+    from vexact_amd import _lib
+
+    lib, p = _lib.load(), 4096
+
+    def call(G, H, pages, B=1):
+        return lib.vx_shared_prefix_attention(p, p, p, p, p, p, p, p, p, B, G, H, H, 128, 256, 1024, 128, 4096, 256, 128, 4096, 256, 128,
+                                              1024, 128, pages, pages, 16, 1.0, 1 << 62, 0, p + 8, 1 << 62, None)
+
+    assert call(2, 8, 64) == -3  # supported: the workspace is refused, for its alignment
+    for G, H, pages, B in ((1 << 30, 1 << 15, (1 << 27) - 128, 1), ((1 << 31) - 1, 65535, (1 << 27) - 17, 1), (1 << 62, 8, 64, 1), (0, 32767, (1 << 27) - 17, 65535),
+                           (2, 8, 1 << 60, 1), (2, 8, (1 << 60) + 4, 1)):
+        assert call(G, H, pages, B) == -2, (G, H, pages, B)
+        assert lib.vx_shared_prefix_workspace_bytes(B, G, H, H, 256, min(pages, 1 << 59) * 16, min(pages, 1 << 59) * 16) == 0

@@ -13,9 +13,19 @@ static int64_t shared_part_bytes(int64_t num_seqs, int64_t num_groups, int64_t H
   return shared_tiles(num_seqs, num_groups, Hq / Hkv) * Hkv * (max_prefix_len / ATT_CHUNK) * shared_image_floats(16, Dv) * 4;
 }
 
+// Sizes whose workgroups, row numbers and workspace bytes stay within their types; every product is of factors bounded before.
+static bool shared_sizes_ok(int64_t num_seqs, int64_t num_groups, int64_t Hq, int64_t Hkv, int64_t Dv, int64_t max_prefix_len, int64_t max_kv_len) {
+  if (Dv > 256 || Hq / Hkv > 32 || num_seqs > 65535 || Hq > 65535 || num_seqs * Hq > 0x7fffffff || num_groups > 0x7fffffff || max_kv_len > 0x7fffff00)
+    return false;
+  const int64_t tiles = shared_tiles(num_seqs, num_groups, Hq / Hkv) * Hkv;
+  return tiles <= 0x7fffffff / (max_prefix_len / ATT_CHUNK + 8) &&  // workgroups
+         num_seqs * Hkv <= ((int64_t)1 << 40) / ((max_kv_len + ATT_CHUNK - 1) / ATT_CHUNK);  // own images, below 2^16 bytes each
+}
+
 int64_t vx_shared_prefix_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t Hq, int64_t Hkv, int64_t Dv, int64_t max_prefix_len,
                                          int64_t max_kv_len) {
   if (num_seqs <= 0 || num_groups < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Dv <= 0 || max_prefix_len < 0 || max_kv_len <= 0) return 0;
+  if (!shared_sizes_ok(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len, max_kv_len)) return 0;
   return shared_part_bytes(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len) +
          num_seqs * Hkv * ((max_kv_len + ATT_CHUNK - 1) / ATT_CHUNK) * shared_image_floats(Hq / Hkv, Dv) * 4;
 }
@@ -34,12 +44,12 @@ int vx_shared_prefix_attention(const void* q, const void* k, const void* v, void
   if (Dk > 256 || Dv > 256 || Hq / Hkv > 32 || num_seqs > 65535 || Hq > 65535) return VX_ERR_UNSUPPORTED;
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 2 != 0) return VX_ERR_ARG;
   if (num_seqs == 0) return VX_OK;
+  if (max_pages > 0x7fffff00 / page_size) return VX_ERR_UNSUPPORTED;
   const int64_t max_kv = max_pages * (int64_t)page_size;
   if (max_prefix_len > max_kv) max_prefix_len = max_kv;
+  if (!shared_sizes_ok(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len, max_kv)) return VX_ERR_UNSUPPORTED;
   const int64_t shared_bytes = shared_part_bytes(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len);
   const int64_t need = vx_shared_prefix_workspace_bytes(num_seqs, num_groups, Hq, Hkv, Dv, max_prefix_len, max_kv);
-  if (num_groups > 0x7fffffff || max_kv > 0x7fffff00 || num_seqs * Hq > 0x7fffffff) return VX_ERR_UNSUPPORTED;
-  if (shared_tiles(num_seqs, num_groups, Hq / Hkv) * Hkv * (max_prefix_len / ATT_CHUNK + 8) > 0x7fffffff) return VX_ERR_UNSUPPORTED;  // workgroups
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) return VX_ERR_WORKSPACE;
   // rows that 16-byte accesses cannot address go element by element
   const bool elem = (sqt | sqh | skb | skp | skh | svb | svp | svh | sot | soh | (int64_t)Dk | (int64_t)Dv) % 8 != 0 ||
