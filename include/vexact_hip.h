@@ -112,7 +112,7 @@ int vx_logprobs_static(const void* logits, const int64_t* labels, float* out, in
  * logit is rounded to bf16 once before the two products, which accumulate in fp32; no atomics, results repeat bit for
  * bit. H up to 2^22, row pitches of hidden and weight 0 (one row for all) to 2^22 elements. The backward takes
  * T * min(8192, V rounded up to 64) < 2^31 - 8192 (262142 rows from V = 8129 on), 8192 max(ldw, H) + H < 2^31 and
- * T H < 2^41; its workspace function returns 0 for sizes that it does not take (with ldw <= H). */
+ * T H < 2^34 - 1023; its workspace function returns 0 for sizes that it does not take (with ldw <= H). */
 int64_t vx_vocab_logprobs_workspace_bytes(int64_t T, int64_t V);
 int vx_vocab_logprobs(const void* hidden, const void* weight, const int64_t* labels, float* out, float* lse, int64_t T,
                       int64_t V, int64_t H, int64_t ldh, int64_t ldw, float scale, void* workspace,

@@ -440,6 +440,16 @@ def test_c_abi_backward_limits():
         assert lib.vx_vocab_logprobs_bwd_workspace_bytes(T, V, H) == 0 and bwd(T, V, H) == -2, (T, V, H)
 
 
+def test_c_abi_backward_grid_limit():
+    """Four elements of d_hidden per thread, fewer than 2^32 threads in a launch."""
+    from vexact_amd import _lib
+
+    lib, a = _lib.load(), 4096
+    for T, H, rc in ((262142, 65536, -3), (262142, 65544, -2), (100000, 1 << 17, -3), (100000, 200000, -2)):
+        assert (lib.vx_vocab_logprobs_bwd_workspace_bytes(T, 9000, H) > 0) == (rc == -3), (T, H)
+        assert lib.vx_vocab_logprobs_bwd(a, a, a, a, a, a, a, T, 9000, H, H, H, H, H, 1.0, a, 16, None) == rc, (T, H)
+
+
 @gpu
 def test_most_rows():
     """As many rows as the backward takes, offsets up to 2^32; one more is refused by the differentiable forward already."""

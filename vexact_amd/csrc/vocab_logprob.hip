@@ -282,10 +282,10 @@ static VocabPlan vocab_plan(int64_t T, int64_t V, int64_t H, int64_t ldw) {
   return q;
 }
 
-// whether the products over a piece stay within their kernels' 32-bit offsets and grids
+// whether the products over a piece stay within their kernels' 32-bit offsets, and vocab_dh_kernel's grid below 2^32 threads
 static bool vocab_plan_fits(const VocabPlan& q, int64_t T, int64_t H, int64_t ldw) {
   const int64_t lim = (int64_t)1 << 32;
-  return (T * q.ld + VL_SEG) * 2 < lim && (q.per * VL_SEG * ldw + H) * 2 < lim && (T * H / 4 + 255) / 256 <= 0x7fffffff;
+  return (T * q.ld + VL_SEG) * 2 < lim && (q.per * VL_SEG * ldw + H) * 2 < lim && T * H / 4 <= 0xffffff00;
 }
 
 }  // namespace vx

@@ -343,7 +343,7 @@ def _vocab_backward_bytes(x, w) -> int:
     (T, H), V = x.shape, w.shape[0]
     nbytes = _lib.load().vx_vocab_logprobs_bwd_workspace_bytes(T, V, H)
     if nbytes == 0 and T > 0:
-        raise ValueError(f"vocab_logprobs: T * min(8192, V rounded up to 64) must be below 2^31 - 8192, 8193 H below 2^31 and T H below 2^41 "
+        raise ValueError(f"vocab_logprobs: T * min(8192, V rounded up to 64) must be below 2^31 - 8192, 8193 H below 2^31 and T H below 2^34 - 1023 "
                          f"for the backward, got T = {T}, V = {V}, H = {H}")
     return nbytes
 
