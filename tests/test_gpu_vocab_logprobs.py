@@ -425,6 +425,47 @@ def test_c_abi_refuses_scales_out_of_range():
         assert lib.vx_vocab_logprobs(a, a, a, a, a, 4, 10, 16, 16, 16, scale, a, 16, None) == -3
 
 
+# d_hidden by 256 x 256 tiles (what more than 1152 workgroups of 64 or 96 rows x 64 columns x 8192 tokens come to, per round of
+# 256 tiles): segments that end inside a step of 64 tokens, a last segment of 10 tokens, one segment that is shorter than a step,
+# a depth that ends inside a tile, several pieces of several segments
+WIDE = [(3000, 20011, 1024), (3001, 8202, 1536), (6000, 50, 1536), (3000, 20011, 1000), (12000, 40001, 512)]
+
+
+@gpu
+@pytest.mark.parametrize("T,V,H", WIDE)
+def test_backward_of_large_batches(T, V, H):
+    h, w, y = (t.cuda() for t in make(T, V, H, seed=T + 7, ignored=T // 7))
+    d = torch.randn(T, generator=torch.Generator().manual_seed(3)).cuda()
+    _, lse = ops.vocab_logprobs(h, w, y, 1.3)
+    dh, dw = ops.vocab_logprobs_backward(h, w, y, lse, d, 1.3)
+    _, _, dx, dh_ref, dw_ref = reference(h, w, y, 1.3, d)
+    slack = 2.0**-8 + 2.0**-11
+    assert ((dh.double() - dh_ref).abs() <= slack * (dx.abs() @ w.double().abs()) + 2.0**-8 * dh_ref.abs() + 1e-30).all()
+    assert ((dw.double() - dw_ref).abs() <= slack * (dx.abs().t() @ h.double().abs()) + 2.0**-8 * dw_ref.abs() + 1e-30).all()
+    assert not dh[(y < 0)].any()
+    again = ops.vocab_logprobs_backward(h, w, y, lse, d, 1.3)
+    assert_bitwise(again[0], dh, "d_hidden again")
+    assert_bitwise(again[1], dw, "d_weight again")
+    # small batches take other kernels (tiles of 64 and 96 rows): the same bits
+    for a, b in ((0, 1), (250, 350), (T - 257, T)):
+        few = ops.vocab_logprobs_backward(h[a:b], w, y[a:b], lse[a:b], d[a:b], 1.3, need_weight=False)[0]
+        assert_bitwise(few, dh[a:b], f"d_hidden of rows {a}..{b}")
+
+
+@gpu
+@pytest.mark.parametrize("T", [16500, 33000])
+def test_rows_in_several_launches(T):
+    """Rows 256 KB apart, more than 4 GiB of them: the logits of a launch reach as far as its 32-bit offsets."""
+    V, H, pitch = 300, 64, 1 << 17
+    h, w, y = (t.cuda() for t in make(T, V, H, seed=41, ignored=9))
+    far = torch.empty(T, pitch, dtype=h.dtype, device="cuda")[:, :H].copy_(h)
+    assert far.stride(0) == pitch and T * pitch * 2 > 1 << 32
+    d = torch.linspace(-1, 1, T).cuda()
+    near, apart = ops.vocab_logprobs(h, w, y), ops.vocab_logprobs(far, w, y)
+    for a, b in zip(near + ops.vocab_logprobs_backward(h, w, y, near[1], d), apart + ops.vocab_logprobs_backward(far, w, y, near[1], d)):
+        assert_bitwise(a, b)
+
+
 def test_c_abi_backward_limits():
     """The workspace function says which sizes the backward takes, and the backward agrees."""
     from vexact_amd import _lib
