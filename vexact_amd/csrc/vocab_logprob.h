@@ -10,7 +10,7 @@
 // row's bits depend on its own hidden state only. The logits stay in fp32 from the accumulator on; what the framework
 // computes from a [T, V] tensor of logits rounds them to that tensor's type first.
 // Backward: the same product again with the derivative as its epilogue, rounded to bf16 once, as the operand of the
-// two products that follow (half a step, 2^-9 relative, of each entry; their sums are in fp32).
+// two products that follow (up to half a step, 2^-8 relative, of each entry; their sums are in fp32).
 #pragma once
 #include "gemm_core.h"
 

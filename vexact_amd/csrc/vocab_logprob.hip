@@ -259,7 +259,8 @@ static inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // The backward's piece: segments per piece so that the piece and its partial sums stay near 768 MB (the whole
 // vocabulary at once up to some hundred rows, one segment at a time from some ten thousand) and the piece's weights
-// within the kernels' 32-bit offsets.
+// within the kernels' 32-bit offsets. Rows are never split (d W is one chain over them), so from there on the workspace grows
+// with them, T (16384 + 10 H) bytes: 1.0 GB at 16384 rows of H 2048, 2.4 GB at 65536.
 struct VocabPlan {
   int64_t segs, per, pieces, ld;  // segments of the vocabulary, of a piece; pieces; columns of the piece buffer
   int64_t dlog_bytes, part_bytes, acc_bytes, rows_bytes;
