@@ -392,7 +392,7 @@ int vx_router_topk_bwd(const void* logits, const int64_t* idx, const void* d_wei
  * consecutive experts scores the sum of its best group_top (1 or 2) c, and experts outside the topk_groups best groups
  * rank as -inf; idx [T, k] = the k largest c in descending order, weights [T, k] = scale * s / (renorm: sum of the
  * selected s; all of them 0: weights 0). Ties go to the lower index, NaN ranks with -inf; scores and sums are held in
- * 64 bits, so the selection is that of the exact scores. E <= 512, k <= 64, n_groups <= 64, topk_groups groups must
+ * 64 bits (sigmoids of logits above 37 are 1 there: a tie). E <= 512, k <= 64, n_groups <= 64, topk_groups groups must
  * hold at least k experts. vx_router_topk is the router of the reference's own block (softmax, no bias, no groups).
  * The backward gives d_logits [T, E] (the logits' type) from idx (int64; an expert named twice in a row has the sum of
  * both derivatives, an index outside [0, E) selects nothing) and d_weights [T, k]. */

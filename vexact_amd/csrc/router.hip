@@ -6,9 +6,13 @@
 // bias, no groups; vexact/models/qwen3_moe/modeling_qwen3_moe.py:128-134).
 // Which of two close scores is larger must not hang on a rounding (a trainer and a rollout have to route alike, and a
 // bias makes near ties common), so scores, biased scores and group scores are held in 64 bits.
-// Bound by the 64-bit exponentials and the k selections, which depend on each other, not by memory: 64 tokens x 256 experts in
-// 8 groups, 8 of them selected, take 8.4 us, 16384 tokens 32 us (0.6 TB/s), their gradient 17 us (2 TB/s). One wavefront
-// per token keeps a row in registers, so every selection is a few cross-lane maxima and no memory is read twice.
+// A decode step (64 tokens x 256 experts in 8 groups, 8 of them selected: 8.4 us) is bound by its eight selections, each of
+// which needs the one before; a large batch by the issue of vector instructions, not by memory: 16384 tokens take 32 us (0.6
+// TB/s) with the vector units at work in 91 % of the busy cycles, their gradient 17 us (2 TB/s) in 81 %. Of a forward call's
+// 30 us the scores (64-bit exponential and division) and the row's loads take 11, the group scores 8 to 10 and a selection 1.1
+// (k = 1 without groups 12.1 us, k = 8 20.1, k = 8 in 8 groups 29.8; softmax 14.6 / 21.9 / 29.5; no renormalisation 27.0 and
+// 28.2 of the last). One wavefront per token keeps a row in registers, so every selection is a few cross-lane maxima and no
+// memory is read twice.
 #include "common.h"
 
 namespace vx {

@@ -944,7 +944,7 @@ def router_topk_grouped(
     """``(weights [T, k], experts [T, k])``: softmax or sigmoid scores, ``bias [E]`` (fp32) added for the selection only, the
     ``topk_groups`` best of ``n_groups`` groups (by the sum of their best ``group_top`` biased scores), the ``top_k`` best
     experts of those in descending order (ties: lower index), weights ``scale * score`` renormalised over the selected.
-    Scores are compared in 64 bits. ``router_topk`` is the router of the reference's own block."""
+    Scores are compared in 64 bits (sigmoids of logits above 37 are 1 there: a tie). ``router_topk`` is the router of the reference's own block."""
     lg = _grouped_router_logits(logits, top_k, score)
     T, E = lg.shape
     if out_dtype not in (torch.float32, torch.bfloat16) or index_dtype not in (torch.int32, torch.int64):
