@@ -261,7 +261,8 @@ int vx_attention_typed(const void* q, const void* k, const void* v, void* out, f
  * prefixes: group g = the sequences group_offsets[g] .. group_offsets[g + 1] - 1 (ascending, int32 on the device), whose
  * block tables name the same pages for their first prefix_lens[g] keys. Whole 256-key chunks of a shared prefix are
  * computed once per group, everything else per sequence; same bits as vx_attention on the same tables. Sequences
- * before the first or behind the last group, and groups of one, share nothing. A sequence without keys gets zeros;
+ * before the first or behind the last group, and groups of one, share nothing. A slot without a query token counts as
+ * empty, whatever its seqused_k and block table hold. A sequence without keys gets zeros;
  * rows of out that belong to no sequence, or to one without a query token, are left as they were. max_prefix_len: an upper
  * bound of prefix_lens that sizes the launch and the workspace (longer prefixes are shared up to it). bf16 (dtype 0) or
  * fp16 (1), head sizes up to 256, Hq / Hkv <= 32, caches as for vx_attention. The workspace holds the chunk states

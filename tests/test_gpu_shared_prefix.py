@@ -166,6 +166,21 @@ def test_no_groups_and_a_given_workspace():
 
 
 @gpu
+def test_the_first_columns_of_a_wide_table():
+    """A view of the columns that are in use gives the same bits, and asks for a workspace of its own width."""
+    a = make([4, 3], [600, 300], [40, 7, 300], (8, 2), (128, 128), 16, seed=15)
+    want, width = paged(a, decode_kernel="split"), a["page_table"].shape[1]
+    wide = torch.full((7, 8192), 1 << 30, dtype=torch.int32).cuda()
+    wide[:, :width] = a["page_table"]
+    assert_bitwise(ops.shared_prefix_attention(**{**a, "page_table": wide}, max_prefix_len=600), want)
+    a["page_table"] = wide[:, :width]
+    assert not a["page_table"].is_contiguous()
+    ws = torch.zeros(4 << 20, dtype=torch.uint8, device="cuda")
+    assert_bitwise(ops.shared_prefix_attention(**a, max_prefix_len=600, workspace=ws), want)
+    assert ws.any()
+
+
+@gpu
 def test_a_full_decode_batch():
     a = make([16] * 16, [1024 + 96 * i for i in range(16)], list(range(1, 600, 37)), (32, 4), (128, 128), 16, seed=3, head_major=True)
     assert_bitwise(ops.shared_prefix_attention(**a), paged(a))

@@ -34,7 +34,8 @@ class KVCacheInfo:
 class PrefixGroups:
     """Sequences of a decode step that share the pages of a prefix (answers to one prompt): group ``g`` holds the sequences
     ``offsets[g] .. offsets[g + 1] - 1`` (int32 ``[G + 1]``), whose block tables name the same pages for their first
-    ``lens[g]`` keys (int32 ``[G]``); ``max_len`` bounds ``lens`` from above. No counterpart in the reference."""
+    ``lens[g]`` keys (int32 ``[G]``); ``max_len`` bounds ``lens`` from above (None: the block tables' width, for which the
+    workspace is then made). No counterpart in the reference."""
 
     offsets: torch.Tensor
     lens: torch.Tensor

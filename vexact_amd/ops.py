@@ -742,8 +742,9 @@ def shared_prefix_attention(
     """``paged_attention`` of a decode step (``max_seqlen_q == 1``) whose sequences share long prefixes, same bits: group
     ``g`` holds the sequences ``group_offsets[g] .. group_offsets[g + 1] - 1`` (int32 ``[G + 1]``, ascending), whose block
     tables name the same pages for the first ``prefix_lens[g]`` (int32 ``[G]``) keys; those are read once per group.
-    ``max_prefix_len`` bounds ``prefix_lens`` from above (default: the block table's width); it sizes the launch and the
-    workspace. A sequence without keys gets zeros. bf16 or fp16."""
+    ``max_prefix_len`` bounds ``prefix_lens`` from above (default: the block table's width). It and the table's width size the
+    launch and the workspace (fp32 states of every 256 keys, gigabytes for tables of 100 000 keys): of a table far wider than
+    the longest sequence pass a view of its first columns. A slot without a query token counts as empty. A sequence without keys gets zeros. bf16 or fp16."""
     _need_gpu("q", q)
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4 or page_table.dim() != 2:
         raise ValueError("shared_prefix_attention: need q [tokens, heads, dim], caches [blocks, page, heads, dim] and a 2-D page table")
