@@ -362,6 +362,30 @@ def test_prefix_groups_refuse_nothing_that_runs_without_them(form):
         assert_bitwise(results[1], results[0])
 
 
+@gpu
+def test_prefix_groups_with_buffers_of_more_rows_than_sequences():
+    """Block tables and query offsets longer than the step has sequences, and a value cache of more pages, as without groups."""
+    from types import SimpleNamespace
+
+    from vexact_amd.batch_invariant_ops import flash_attention_forward
+    from vexact_amd.batch_invariant_ops.kv_cache_context import PrefixGroups, clear_kv_cache_context, set_kv_cache_context
+
+    a = make([3, 2], [300, 600], [40, 7], (8, 2), (64, 64), 16, seed=16)
+    table = torch.cat([a["page_table"], torch.full_like(a["page_table"], -1)])
+    cu = torch.cat([a["cu_seqlens_q"], a["cu_seqlens_q"][-1:].expand(6)])
+    for v in (a["v_cache"], torch.cat([a["v_cache"], a["v_cache"]])):
+        outs = []
+        for groups in (None, PrefixGroups(a["group_offsets"], a["prefix_lens"], 600)):
+            set_kv_cache_context(is_paged_attn=True, key_cache={0: a["k_cache"]}, value_cache={0: v}, block_tables=table,
+                                 context_lens=a["seqused_k"], slot_mapping=None, query_start_loc=cu, max_seqlen_q=1, prefix_groups=groups)
+            try:
+                with torch.no_grad():
+                    outs.append(flash_attention_forward(SimpleNamespace(layer_idx=0), a["q"].transpose(0, 1).unsqueeze(0), None, None, None, 0.1)[0])
+            finally:
+                clear_kv_cache_context()
+        assert_bitwise(outs[1], outs[0])
+
+
 def test_refusals():
     z = torch.zeros
     with pytest.raises(ValueError, match="CUDA tensor"):

@@ -196,12 +196,13 @@ def _first_given(kwargs: dict, *names):
     return next((kwargs[n] for n in names if kwargs.get(n) is not None), None)
 
 
-def _reads_prefixes_once(kv_ctx, q, k_blocks, scaling, dropout) -> bool:
+def _reads_prefixes_once(kv_ctx, q, k_blocks, v_blocks, scaling, dropout) -> bool:
     """Whether a step with prefix groups takes ``ops.shared_prefix_attention``: a decode step of what that supports. The groups
     only say that keys may be read once, so everything else runs, or is refused, as it is without them."""
     step = kv_ctx.max_seqlen_q
     return (kv_ctx.prefix_groups is not None and not torch.is_tensor(step) and step == 1 and dropout == 0.0 and not torch.is_tensor(scaling)
-            and not torch.is_grad_enabled() and q.dtype in (torch.bfloat16, torch.float16) and q.shape[1] <= 32 * k_blocks.shape[2])
+            and not torch.is_grad_enabled() and q.dtype in (torch.bfloat16, torch.float16) and q.shape[1] <= 32 * k_blocks.shape[2]
+            and k_blocks.shape[:3] == v_blocks.shape[:3])
 
 
 def flash_attention_forward(
@@ -232,12 +233,12 @@ def flash_attention_forward(
         if have_kv:  # this step's keys and values go into the cache first
             rows = [t if t.stride(-1) == 1 and t.stride(1) == t.shape[-1] else t.contiguous() for t in (k, v)]
             ops.store_kvcache(rows[0], rows[1], k_blocks, v_blocks, kv_ctx.slot_mapping)
-        if _reads_prefixes_once(kv_ctx, q, k_blocks, scaling, dropout):
-            groups = kv_ctx.prefix_groups
-            table = kv_ctx.block_tables if kv_ctx.block_tables.stride(-1) == 1 else kv_ctx.block_tables.contiguous()
+        if _reads_prefixes_once(kv_ctx, q, k_blocks, v_blocks, scaling, dropout):
+            groups, n = kv_ctx.prefix_groups, kv_ctx.context_lens.numel()
+            table = kv_ctx.block_tables[:n]  # static buffers of a step may hold more rows than it has sequences
             return ops.shared_prefix_attention(
-                _addressable(q), k_blocks, v_blocks, kv_ctx.query_start_loc.contiguous(), kv_ctx.context_lens.contiguous(), table,
-                groups.offsets, groups.lens, q.shape[-1] ** -0.5 if scaling is None else float(scaling), max_prefix_len=groups.max_len), None
+                _addressable(q), k_blocks, v_blocks, kv_ctx.query_start_loc[: n + 1].contiguous(), kv_ctx.context_lens.contiguous(),
+                table if table.stride(-1) == 1 else table.contiguous(), groups.offsets, groups.lens, q.shape[-1] ** -0.5 if scaling is None else float(scaling), max_prefix_len=groups.max_len), None
         return flash_attn_varlen_func(
             q, k_blocks, v_blocks, cu_seqlens_q=kv_ctx.query_start_loc, max_seqlen_q=kv_ctx.max_seqlen_q,
             seqused_k=kv_ctx.context_lens, page_table=kv_ctx.block_tables, dropout_p=dropout, softmax_scale=scaling,
